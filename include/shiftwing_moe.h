@@ -555,6 +555,80 @@ int coli_cuda_output_head_q8(ColiCuda *ctx, float *logits, float *hidden,
 int coli_cuda_moe_stack_drill(ColiCuda *ctx, int absent_workgroups,
                               int wait_limit_us);
 
+/* ---- Part 3: paged key-value cache and packed Gated DeltaNet ------------- */
+/* No counterpart in the reference backend, whose caches are one fp32 slab a
+ * slot and whose Gated DeltaNet advances a handful of tokens a call.  The same
+ * conventions: 0 / -1 with a message, device pointers owned by the caller,
+ * everything ordered on the context's stream, nothing waited for.
+ *
+ * Element types of the tensors of this part (sums, softmax statistics and
+ * recurrent states are fp32 whatever the type). */
+enum { COLI_TYPE_F32 = 0, COLI_TYPE_F16 = 1, COLI_TYPE_BF16 = 2 };
+
+/* A cache of fixed-size pages.  The key and the value pool hold `pages` pages
+ * each, [page_size][kv_heads][head_dim], `page_stride` elements from one page
+ * to the next (at least page_size * kv_heads * head_dim; more where both pools
+ * are interleaved).  The page table is device memory, [sequences][table_pages]
+ * ints: position p of sequence s lies in page table[s][p / page_size] at
+ * p % page_size.  Ids outside [0, pages) name no page: positions there are not
+ * written, and attention leaves them out.
+ *
+ * query_heads a multiple of kv_heads; head_dim 64, 128 or 256; pools 16-byte
+ * aligned, page_stride a multiple of 8.  pages * page_size and
+ * table_pages * page_size stay below 2^31. */
+typedef struct {
+  int type; /* COLI_TYPE_*: queries, keys, values, gates, outputs, both pools */
+  int query_heads, kv_heads, head_dim;
+  int page_size, pages, table_pages;
+  long long page_stride;
+} ColiPaged;
+
+/* Packed sequences (host arrays): sequence s owns rows start[s] ..
+ * start[s + 1] - 1 of the token tensors (start ascending from start[0] >= 0,
+ * sequences + 1 entries), and they are the last of its length[s] cached
+ * positions.  Rows of no sequence are neither read nor written.  A sequence
+ * may have no row.
+ *
+ * Appends the rows' keys and values to their pages, position rotation applied
+ * on the way.  A head's vector is normalised first, x / rms(x) * (1 + norm)
+ * with eps, where its norm is given (as the mixer layers do; NULL: not); then
+ * dims i and i + rotary_dim / 2 of the first rotary_dim are turned by
+ * position * theta^(-2 i / rotary_dim), an angle held in 64 bits (rotary_dim
+ * even, 0: no rotation).  Queries get the same into q_out
+ * [rows][query_heads][head_dim]; q and q_out are both given or both NULL.
+ * Row strides are elements from token to token, q_head_stride from query head
+ * to query head (2 * head_dim where a gate lies behind each query), key and
+ * value heads are contiguous; q_out must not overlap q. */
+int coli_cuda_paged_append(ColiCuda *ctx, const ColiPaged *cache,
+                           void *k_pool, void *v_pool, const int *table,
+                           const int *start, const int *length, int sequences,
+                           void *q_out, const void *q, long long q_stride,
+                           int q_head_stride, const void *k,
+                           long long k_stride, const void *v,
+                           long long v_stride, const float *q_norm,
+                           const float *k_norm, float eps, int rotary_dim,
+                           float theta);
+/* Attention of one new token a sequence: out[s] [query_heads][head_dim] =
+ * softmax(scale * q[s] . k_j) v_j over positions j < length[s] (host array) of
+ * the cache, query head h on kv head h / (query_heads / kv_heads), times
+ * sigmoid(gate) where gates are given (gate_stride elements from row to row,
+ * gate_head_stride from head to head, both multiples of 4).  q and out are
+ * contiguous and 16-byte aligned.  Sequences that see nothing get zeros. */
+int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *cache, void *out,
+                           const void *q, const void *gate,
+                           long long gate_stride, int gate_head_stride,
+                           const void *k_pool, const void *v_pool,
+                           const int *table, const int *length, int sequences,
+                           float scale);
+/* The same for packed prompts (or chunks of them, or drafted tokens): row i of
+ * the n rows of a sequence sees its positions up to length - n + i. */
+int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *cache, void *out,
+                           const void *q, const void *gate,
+                           long long gate_stride, int gate_head_stride,
+                           const void *k_pool, const void *v_pool,
+                           const int *table, const int *start,
+                           const int *length, int sequences, float scale);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,9 +24,14 @@ class ColiMoeShape(C.Structure):
                 ("expert_format", C.c_int), ("group_size", C.c_int)]
 
 
+class ColiPaged(C.Structure):
+    _fields_ = [("type", C.c_int), ("query_heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("page_size", C.c_int), ("pages", C.c_int), ("table_pages", C.c_int), ("page_stride", C.c_longlong)]
+
+
 _SCALARS = {
     "int": C.c_int, "float": C.c_float, "size_t": C.c_size_t, "void": None,
-    "unsigned long long": C.c_ulonglong, "double": C.c_double,
+    "unsigned long long": C.c_ulonglong, "long long": C.c_longlong, "double": C.c_double,
 }
 
 

@@ -1,0 +1,1092 @@
+// The paged key-value cache: appending keys and values with the position
+// rotation applied on the way (coli_cuda_paged_append), attention of single new
+// tokens (coli_cuda_paged_decode) and of packed prompts (coli_cuda_paged_prompt).
+//
+// Attention, both forms: o = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - m) over the
+// visible positions j, s_j = scale log2(e) q . k_j, with the running maximum m, the
+// sum and o held in fp32 and rescaled when m grows, so the cache is read once.
+// p is rounded to the cache's 16-bit type for the second product (2^-8 / 2^-11
+// relative a term, what the values themselves carry); an fp32 cache keeps fp32
+// products throughout.
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <math.h>
+#include <string.h>
+
+#include "sw_lds_dma.h"
+#include "sw_serve.h"
+
+namespace sw {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Where a sequence's positions lie.  Offsets are 64-bit: a pool may hold more
+// than 2^31 elements.
+struct PageMap {
+  const int *table;  // [sequence][table_pages]
+  int pages, table_pages, page_size;
+  FastDiv div;  // by page_size
+  long long stride;
+  int row;  // elements of one position: kv_heads * head_dim
+};
+// Element offset of position p of the sequence whose table row is `tab`; -1 where
+// the table names no page.
+__device__ __forceinline__ long long cell(const PageMap &m, const int *tab, int p) {
+  const int pg = div_by(m.div, p);
+  const int id = tab[pg];
+  return (unsigned)id < (unsigned)m.pages ? (long long)id * m.stride + (long long)(p - pg * m.page_size) * m.row : -1;
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+struct AppendArgs {
+  const void *q, *k, *v;
+  void *q_out, *k_pool, *v_pool;
+  long long q_stride, k_stride, v_stride;
+  const float *q_norm, *k_norm;
+  int q_head, nh, nkv, rd, heads_per_block, seqs, first_seq;
+  float eps;
+  PageMap map;
+  double freq[128];  // turns a position
+  int start[kSeqs + 1], len[kSeqs];
+};
+
+template <class T, int E>
+struct alignas(sizeof(T) * E) Pack {
+  T v[E];
+};
+
+// One workgroup a (token, run of heads), one wave a head: E = HD / 64 elements a
+// lane.  HBM-bound (each value read and written once).  The angle is formed once a
+// workgroup: turns = position * freq in 64 bits, the whole turns dropped, the rest
+// to fp32 (2^-25 turns), so far positions keep theirs.  The rotation's partners meet
+// in LDS, where any even rotary_dim finds them.
+template <class T, int HD>
+__global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
+  constexpr int E = HD / 64;
+  typedef Pack<T, E> P;
+  __shared__ float s_co[128], s_si[128], s_row[4][HD];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int t = a.start[0] + blockIdx.x;
+  const int s = find_span(a.start, a.seqs, t);
+  const int pos = a.len[s] - a.start[s + 1] + t;
+  const int half = a.rd >> 1, nq = a.q ? a.nh : 0;
+  for (int i = threadIdx.x; i < half; i += 256) {
+    double turns = (double)pos * a.freq[i];
+    turns -= __builtin_rint(turns);
+    float si, co;
+    sincospif(2.0f * (float)turns, &si, &co);
+    s_co[i] = co;
+    s_si[i] = si;
+  }
+  __syncthreads();
+  const long long at = cell(a.map, a.map.table + (size_t)(a.first_seq + s) * a.map.table_pages, pos);
+  const int h1 = min(nq + a.nkv, (int)(blockIdx.y + 1) * a.heads_per_block);
+  for (int h = blockIdx.y * a.heads_per_block + wave; h < h1; h += 4) {
+    const bool isq = h < nq;
+    const int kvh = h - nq;
+    const T *src = isq ? (const T *)a.q + (size_t)t * a.q_stride + (size_t)h * a.q_head
+                       : (const T *)a.k + (size_t)t * a.k_stride + (size_t)kvh * HD;
+    if (!isq && at < 0) continue;
+    const P in = *(const P *)(src + E * lane);
+    P vin;
+    if (!isq) vin = *(const P *)((const T *)a.v + (size_t)t * a.v_stride + (size_t)kvh * HD + E * lane);
+    float x[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) x[e] = (float)in.v[e];
+    const float *norm = isq ? a.q_norm : a.k_norm;
+    if (norm) {
+      float s2 = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; e++) s2 = __builtin_fmaf(x[e], x[e], s2);
+      const float r = 1.0f / sqrtf(wave_sum_dpp(s2) / (float)HD + a.eps);
+#pragma unroll
+      for (int e = 0; e < E; e++) x[e] = x[e] * r * (1.0f + norm[E * lane + e]);
+    }
+    float *row = s_row[wave];
+#pragma unroll
+    for (int e = 0; e < E; e++) row[E * lane + e] = x[e];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int j = E * lane + e;
+      if (j < a.rd) {
+        const int i = j < half ? j : j - half;
+        const float lo = row[i], hi = row[i + half], co = s_co[i], si = s_si[i];
+        x[e] = j < half ? __builtin_fmaf(lo, co, -(hi * si)) : __builtin_fmaf(hi, co, lo * si);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    P out;
+#pragma unroll
+    for (int e = 0; e < E; e++) out.v[e] = (T)x[e];
+    if (isq) {
+      *(P *)((T *)a.q_out + ((size_t)t * a.nh + h) * HD + E * lane) = out;
+    } else {
+      *(P *)((T *)a.k_pool + at + (size_t)kvh * HD + E * lane) = out;
+      *(P *)((T *)a.v_pool + at + (size_t)kvh * HD + E * lane) = vin;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// attention of one new token a sequence
+// ---------------------------------------------------------------------------
+struct DecodeArgs {
+  const void *q, *gate, *k, *v;
+  void *out;
+  float *po, *pm, *pl;  // partial records (null: every row has one split)
+  long long gate_stride;
+  int gate_head, nh, nkv, G, hgroups, rows, first_seq, per;
+  float scale;  // scale * log2(e)
+  PageMap map;
+  int first[kSeqs + 1], len[kSeqs];  // row r's splits are first[r] .. first[r + 1] - 1
+};
+
+__device__ __forceinline__ v4f mfma_f32_16(float a, float b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// One workgroup of 4 waves a (sequence, split of its positions, kv head, group of
+// 16 query heads); a wave takes every fourth block of KB positions.  The scores
+// come transposed, S^T (positions x heads) = K Q^T, so that a lane holds one head's
+// probabilities of the positions 4 kg + i whose values it also loads: the second
+// product O^T (dims x heads) += V^T P^T takes them as they are.  Its A operand wants
+// consecutive positions of one dim where memory has consecutive dims of one
+// position: in 16 bits a lane loads 8 dims of 8 positions and regroups them by byte
+// permutes (16 to 16 loaded registers), an fp32 lane's value is the operand itself;
+// row n of dim tile d stands for dim W n + d (tiles of one load).
+// Nothing goes through LDS until the waves' merge.  HBM-bound.
+// RUN16: pages hold whole runs of 16 positions, whose page the wave then looks up
+// once, by a scalar load; otherwise every lane looks up its own positions.
+template <class T, int HD, bool RUN16>
+__global__ __launch_bounds__(256) void k_paged_decode(DecodeArgs a) {
+  constexpr bool B16 = sizeof(T) == 2;
+  constexpr int NB = B16 ? 2 : 1, KB = 16 * NB;            // runs and positions of a block
+  constexpr int NT = HD / 16;                              // dim tiles
+  constexpr int KR = HD * (int)sizeof(T) / 64;             // registers x 4 of a run's keys
+  constexpr int W = B16 ? (HD >= 128 ? 8 : 4) : 4;         // values of one load
+  constexpr int NW = NT / W;                               // loads of one position
+  constexpr int LV = W * (int)sizeof(T) / 4;               // registers of one load
+  __shared__ float s_m[4][16], s_l[4][16], s_lsum[16];
+  __shared__ float s_o[16 * (HD + 1)];
+  __shared__ v4u s_q[B16 ? 1 : KR * 64];                   // fp32: [chunk][lane]
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  const int per_split = a.nkv * a.hgroups;
+  const int slot = blockIdx.x / per_split, sub = blockIdx.x % per_split;
+  const int kvh = sub / a.hgroups, hg = sub % a.hgroups;
+  const int r = find_span(a.first, a.rows, slot);
+  const int len = a.len[r];
+  const int heads = min(16, a.G - 16 * hg), h0 = kvh * a.G + 16 * hg;
+  const int key_first = (slot - a.first[r]) * a.per, key_end = min(len, key_first + a.per);
+  const int *tab = a.map.table + (size_t)(a.first_seq + r) * a.map.table_pages;
+  const T *kc = (const T *)a.k + (size_t)kvh * HD, *vc = (const T *)a.v + (size_t)kvh * HD;
+
+  // the queries: B operand of the first product; heads beyond the group are zero
+  v4u qv[B16 ? KR : 1];
+  {
+    const T *qrow = (const T *)a.q + ((size_t)r * a.nh + h0 + n) * HD;
+    if constexpr (B16) {
+#pragma unroll
+      for (int i = 0; i < KR; i++) qv[i] = n < heads ? *(const v4u *)(qrow + 32 * i + 8 * kg) : v4u{0, 0, 0, 0};
+    } else {
+      for (int i = wave; i < KR; i += 4)
+        s_q[i * 64 + lane] = n < heads ? *(const v4u *)(qrow + 16 * i + 4 * kg) : v4u{0, 0, 0, 0};
+      __syncthreads();
+    }
+  }
+  v4f o[NT];
+#pragma unroll
+  for (int d = 0; d < NT; d++) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  for (int key0 = key_first + wave * KB; key0 < key_end; key0 += 4 * KB) {
+    // keys 16 b + n (A operand) and values of positions 16 b + 4 kg + j; a position
+    // that is not there reads the first cell of the pool and is masked below
+    v4u kr[NB][KR];
+    unsigned vr[NB][4][NW][LV];
+    bool there[NB][4];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      const int p0 = key0 + 16 * b;
+      long long base = -1;
+      if (RUN16) {
+        const int u0 = __builtin_amdgcn_readfirstlane(p0);
+        if (u0 < key_end) base = cell(a.map, tab, u0);
+      }
+      long long ck, cv[4];
+      if (RUN16) {
+        ck = base >= 0 && p0 + n < key_end ? base + (long long)n * a.map.row : -1;
+      } else {
+        ck = p0 + n < key_end ? cell(a.map, tab, p0 + n) : -1;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int p = p0 + 4 * kg + j;
+        if (RUN16)
+          cv[j] = base >= 0 && p < key_end ? base + (long long)(4 * kg + j) * a.map.row : -1;
+        else
+          cv[j] = p < key_end ? cell(a.map, tab, p) : -1;
+        there[b][j] = cv[j] >= 0;
+      }
+      const T *kp = kc + (ck >= 0 ? ck : 0);
+#pragma unroll
+      for (int i = 0; i < KR; i++) kr[b][i] = *(const v4u *)(kp + (64 / sizeof(T)) * i + (16 / sizeof(T)) * kg);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const T *vp = vc + (cv[j] >= 0 ? cv[j] : 0) + W * n;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+          if constexpr (LV == 4) {
+            const v4u x = *(const v4u *)(vp + 16 * W * w);
+#pragma unroll
+            for (int e = 0; e < 4; e++) vr[b][j][w][e] = x[e];
+          } else {
+            const v2u x = *(const v2u *)(vp + 16 * W * w);
+            vr[b][j][w][0] = x[0];
+            vr[b][j][w][1] = x[1];
+          }
+        }
+      }
+    }
+    // every load of the block is in flight before the first product
+    asm volatile("" ::: "memory");
+    // values behind the end may be anything (0 * NaN is NaN): they become zero
+    bool whole = true;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) whole &= there[b][j];
+    if (!__all(whole)) {
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int w = 0; w < NW; w++)
+#pragma unroll
+            for (int e = 0; e < LV; e++) vr[b][j][w][e] = there[b][j] ? vr[b][j][w][e] : 0u;
+    }
+    float sv[NB][4];
+    float bm = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      v4f sc;
+      if constexpr (B16) {
+        v4f c0 = v4f{0.f, 0.f, 0.f, 0.f}, c1 = c0;
+#pragma unroll
+        for (int i = 0; i < KR; i += 2) {
+          c0 = Mat16<T>::mul16(kr[b][i], qv[i], c0);
+          c1 = Mat16<T>::mul16(kr[b][i + 1], qv[i + 1], c1);
+        }
+        sc = c0 + c1;
+      } else {
+        v4f c[4] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int i = 0; i < KR; i++) {
+          const v4u qq = s_q[i * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; e++) c[e] = mfma_f32_16(__uint_as_float(kr[b][i][e]), __uint_as_float(qq[e]), c[e]);
+        }
+        sc = (c[0] + c[1]) + (c[2] + c[3]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        sv[b][j] = there[b][j] ? sc[j] * a.scale : -INFINITY;
+        bm = fmaxf(bm, sv[b][j]);
+      }
+    }
+    bm = fmaxf(bm, __shfl_xor(bm, 16));
+    bm = fmaxf(bm, __shfl_xor(bm, 32));
+    const float m_new = fmaxf(m_run, bm), m_use = m_new == -INFINITY ? 0.0f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+    float ps = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        sv[b][j] = __builtin_amdgcn_exp2f(sv[b][j] - m_use);
+        ps += sv[b][j];
+      }
+    ps += __shfl_xor(ps, 16);
+    ps += __shfl_xor(ps, 32);
+    l_run = __builtin_fmaf(l_run, alpha, ps);
+    m_run = m_new;
+#pragma unroll
+    for (int d = 0; d < NT; d++) o[d] *= alpha;
+    if constexpr (B16) {
+      const v4u pf = v4u{pack2<T>(sv[0][0], sv[0][1]), pack2<T>(sv[0][2], sv[0][3]), pack2<T>(sv[1][0], sv[1][1]),
+                         pack2<T>(sv[1][2], sv[1][3])};
+#pragma unroll
+      for (int d = 0; d < NT; d++) {
+        const int w = d / W, e = (d % W) / 2;
+        const unsigned sel = d % 2 ? 0x07060302u : 0x05040100u;
+        v4u vf;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          vf[2 * b] = __builtin_amdgcn_perm(vr[b][1][w][e], vr[b][0][w][e], sel);
+          vf[2 * b + 1] = __builtin_amdgcn_perm(vr[b][3][w][e], vr[b][2][w][e], sel);
+        }
+        o[d] = Mat16<T>::mul16(vf, pf, o[d]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int d = 0; d < NT; d++) o[d] = mfma_f32_16(__uint_as_float(vr[0][j][d / W][d % W]), sv[0][j], o[d]);
+    }
+  }
+
+  // the waves meet in LDS, in wave order
+  if (kg == 0) {
+    s_m[wave][n] = m_run;
+    s_l[wave][n] = l_run;
+  }
+  __syncthreads();
+  float M = s_m[0][n];
+#pragma unroll
+  for (int w = 1; w < 4; w++) M = fmaxf(M, s_m[w][n]);
+  const float f = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - M);
+  for (int w = 0; w < 4; w++) {
+    if (wave == w) {
+#pragma unroll
+      for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float *p = s_o + (size_t)n * (HD + 1) + 16 * W * (d / W) + W * (4 * kg + i) + d % W;
+          *p = w == 0 ? o[d][i] * f : __builtin_fmaf(o[d][i], f, *p);
+        }
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x < 16) {
+    float L = 0.0f;
+    for (int w = 0; w < 4; w++)
+      if (s_m[w][n] != -INFINITY) L = __builtin_fmaf(s_l[w][n], __builtin_amdgcn_exp2f(s_m[w][n] - M), L);
+    s_lsum[n] = L;
+    if (a.po && n < heads) {
+      a.pm[(size_t)slot * a.nh + h0 + n] = M;
+      a.pl[(size_t)slot * a.nh + h0 + n] = L;
+    }
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < heads * HD; u += 256) {
+    const int h = u / HD, d = u % HD;
+    const float x = s_o[h * (HD + 1) + d];
+    if (a.po) {
+      a.po[((size_t)slot * a.nh + h0 + h) * HD + d] = x;
+      continue;
+    }
+    float y = s_lsum[h] > 0.0f ? x / s_lsum[h] : s_lsum[h] == 0.0f ? 0.0f : s_lsum[h];  // NaN stays
+    if (a.gate) y *= gate_sigmoid((float)((const T *)a.gate)[(size_t)r * a.gate_stride + (size_t)(h0 + h) * a.gate_head + d]);
+    ((T *)a.out)[((size_t)r * a.nh + h0 + h) * HD + d] = (T)y;
+  }
+}
+
+// Joins the splits of one (row, query head): the weights 2^(m - M) in LDS, then
+// 256 / HD groups of threads sum every NG-th split, eight loads in flight, and
+// meet in LDS in group order.  grid (query heads, rows), S <= kMaxSplits.
+constexpr int kMaxSplits = 256;
+struct JoinArgs {
+  const float *po, *pm, *pl;
+  const void *gate;
+  void *out;
+  long long gate_stride;
+  int gate_head, nh, flat;
+  int S, step;       // not flat: record of split s of row t is s * step + t
+  long long row0;    // first row of out and gate
+  int first[kSeqs + 1];  // flat: row r's records
+};
+template <class T, int HD>
+__global__ __launch_bounds__(256) void k_paged_join(JoinArgs a) {
+  constexpr int NG = 256 / HD;
+  __shared__ float s_w[kMaxSplits], s_red[8], s_o[NG][HD];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = blockIdx.x, t = blockIdx.y;
+  const int S = a.flat ? a.first[t + 1] - a.first[t] : a.S;
+  const size_t base = a.flat ? (size_t)a.first[t] : (size_t)t, step = a.flat ? 1 : (size_t)a.step;
+  const size_t rec = ((base + (size_t)(tid < S ? tid : 0) * step) * a.nh) + h;
+  const float m = tid < S ? a.pm[rec] : -INFINITY, lv = tid < S ? a.pl[rec] : 0.0f;
+  const float wm = wave_max_dpp(m);
+  if (lane == 0) s_red[wave] = wm;
+  __syncthreads();
+  const float M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+  s_w[tid] = w;
+  const float ls = wave_sum_dpp(w == 0.0f ? 0.0f : lv * w);
+  if (lane == 0) s_red[4 + wave] = ls;
+  __syncthreads();
+  const float L = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+  const int d = tid % HD, g = tid / HD;
+  float o = 0.0f;
+  for (int s0 = g; s0 < S; s0 += 8 * NG) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int s = s0 + k * NG;
+      x[k] = a.po[((base + (size_t)(s < S ? s : g) * step) * a.nh + h) * HD + d];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int s = s0 + k * NG;
+      // a record without a visible position holds nothing
+      if (s < S && s_w[s] != 0.0f) o = __builtin_fmaf(x[k], s_w[s], o);
+    }
+  }
+  s_o[g][d] = o;
+  __syncthreads();
+  if (g) return;
+#pragma unroll
+  for (int k = 1; k < NG; k++) o += s_o[k][d];
+  const size_t row = (size_t)a.row0 + t;
+  float y = L > 0.0f ? o / L : L == 0.0f ? 0.0f : L;
+  if (a.gate) y *= gate_sigmoid((float)((const T *)a.gate)[row * a.gate_stride + (size_t)h * a.gate_head + d]);
+  ((T *)a.out)[(row * a.nh + h) * HD + d] = (T)y;
+}
+
+// ---------------------------------------------------------------------------
+// attention of packed prompts
+// ---------------------------------------------------------------------------
+struct PromptArgs {
+  const void *q, *gate, *k, *v;
+  void *out;
+  float *po, *pm, *pl;  // partial records [split][row - row0][head] (null: one split)
+  long long gate_stride;
+  int gate_head, nh, nkv, G, seqs, first_seq, splits, rows;
+  float scale;  // scale * log2(e)
+  FastDiv by_group;
+  PageMap map;
+  int start[kSeqs + 1], len[kSeqs], tile0[kSeqs + 1];  // sequence s's tiles are tile0[s] .. tile0[s + 1] - 1
+};
+
+__device__ float g_zero_row[256];  // never written: what copies of absent positions read
+
+__device__ __forceinline__ v16f mfma_f32_32(float a, float b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+
+// LDS by its 32-bit address
+typedef short v4s __attribute__((ext_vector_type(4)));
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"
+__device__ __forceinline__ v4u lds_v4u(unsigned at) { return *(__attribute__((address_space(3))) const v4u *)at; }
+__device__ __forceinline__ float lds_f32(unsigned at) { return *(__attribute__((address_space(3))) const float *)at; }
+// 16 lanes read four rows x 16 columns, four 16-bit values a lane, and get the four
+// rows of one column each
+__device__ __forceinline__ v2u lds_transposed(unsigned at) {
+  return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)at));
+}
+#pragma clang diagnostic pop
+
+template <class T, int HD>
+struct PromptShape {
+  static constexpr bool B16 = sizeof(T) == 2;
+  static constexpr int kWaves = 4;
+  static constexpr int kKeys = B16 ? 64 : 32;               // positions of a tile
+  static constexpr int kRowBytes = HD * (int)sizeof(T);
+  static constexpr int kTileBytes = kKeys * kRowBytes;      // of one matrix
+  static constexpr int kLds = 4 * kTileBytes + 16;          // K and V, two buffers, flags
+  static constexpr int kRows = 32 * kWaves;                 // (token, head) rows of a workgroup
+  static constexpr int kPerCu = kLds <= 80 * 1024 ? 2 : 1;  // workgroups that a compute unit holds
+};
+
+// One workgroup a (tile of rows, kv head, split of the tile's positions).  A row is
+// one (token, query head of the kv head's group), tokens in order, so that a tile's
+// heads share every key and value it reads; a wave has 32 rows, the columns of its
+// 32x32 matrix instructions.  Tiles of kKeys positions go through two LDS buffers,
+// copied straight from the pages (16 bytes a lane from any address), the next tile
+// while one is multiplied: one barrier a tile.  S^T = K Q^T leaves a lane half the
+// tile's scores of one row, so the row's maximum and sum take one exchange between
+// lane l and l + 32, and the probabilities are the second product's B operand as
+// they stand (positions in the order that the first product left them).  Its A
+// operand, V^T, comes from the untransposed tile by the transposing LDS load
+// (16 bits) or as single values (fp32).
+// LDS rows are stored with their 16-byte chunks exchanged by an XOR with the row
+// number, which spreads every access over all banks.
+template <class T, int HD>
+__global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, HD>::kPerCu)) void k_paged_prompt(PromptArgs a) {
+  typedef PromptShape<T, HD> Sh;
+  constexpr bool B16 = Sh::B16;
+  constexpr int KT = Sh::kKeys, RB = Sh::kRowBytes, CPR = RB / 16, NI = Sh::kTileBytes / 1024 / Sh::kWaves;
+  constexpr int NS = KT / 32;      // 32-position subtiles
+  constexpr int ND = HD / 32;      // 32-dim tiles
+  constexpr int KC = HD * (int)sizeof(T) / 32;  // 16-byte chunks of half a row: Q registers x 4
+  extern __shared__ __align__(1024) unsigned char smem[];
+  // tag of the latest tile of its residue with an absent page: written two tiles
+  // ahead, so four residues keep the tag that others may still read
+  int *s_bad = (int *)(smem + 4 * Sh::kTileBytes);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31,
+            hf = lane >> 5;
+  const int kvh = blockIdx.y, split = blockIdx.z;
+  // late tiles see most and go first
+  const int tile = gridDim.x - 1 - blockIdx.x;
+  const int s = find_span(a.tile0, a.seqs, tile);
+  const int rows = (a.start[s + 1] - a.start[s]) * a.G;        // of the sequence and kv head
+  const int row0 = (tile - a.tile0[s]) * Sh::kRows;
+  const int base = a.len[s] - (a.start[s + 1] - a.start[s]);  // positions before the first row
+  const int *tab = a.map.table + (size_t)(a.first_seq + s) * a.map.table_pages;
+  const T *kc = (const T *)a.k + (size_t)kvh * HD, *vc = (const T *)a.v + (size_t)kvh * HD;
+
+  // the positions of this split
+  const int last_row = min(rows, row0 + Sh::kRows) - 1;
+  const int extent = base + div_by(a.by_group, last_row) + 1;
+  const int per = ((extent + a.splits - 1) / a.splits + KT - 1) / KT * KT;
+  const int key_first = split * per, key_end = min(extent, key_first + per);
+
+  // this lane's row
+  const int row = row0 + 32 * wave + c;
+  const bool live = row < rows;
+  const int tok = div_by(a.by_group, live ? row : last_row), head = kvh * a.G + (live ? row : last_row) - tok * a.G;
+  const size_t qrow = (size_t)(a.start[s] + tok) * a.nh + head;
+  const int lim = base + tok;  // the last visible position
+  // of the wave's rows: no mask is needed up to wave_all, nothing is seen after wave_any
+  const int wrow = min(rows - 1, row0 + 32 * wave), wlast = min(rows - 1, row0 + 32 * wave + 31);
+  const int wave_all = base + div_by(a.by_group, wrow), wave_any = base + div_by(a.by_group, wlast);
+
+  v4u qv[KC];
+  {
+    const T *qp = (const T *)a.q + qrow * HD;
+#pragma unroll
+    for (int i = 0; i < KC; i++)
+      qv[i] = live ? *(const v4u *)(qp + (32 / sizeof(T)) * i + (16 / sizeof(T)) * hf) : v4u{0, 0, 0, 0};
+  }
+  v16f o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  // this lane's part of a tile's copies: chunk and row of each of its NI pieces
+  const unsigned lds0 = lds_addr(smem);
+  auto swz = [](int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; };
+  long long at[NI];
+  auto look_up = [&](int key0, int tag) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      const int p = key0 + ((wave * NI + i) * 64 + lane) / CPR;
+      at[i] = p < key_end ? cell(a.map, tab, p) : -1;
+      bad |= p < key_end && at[i] < 0;
+    }
+    if (__ballot(bad) && lane == 0) s_bad[tag & 3] = tag;
+  };
+  auto copy = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      const int u = (wave * NI + i) * 64 + lane, r = u / CPR, ch = (u % CPR) ^ swz(r);
+      const unsigned dst = lds0 + buf * 2 * Sh::kTileBytes + (wave * NI + i) * 1024;
+      const char *z = (const char *)g_zero_row + (16 * ch) % 1024;
+      dma_b128(at[i] >= 0 ? (const char *)(kc + at[i]) + 16 * ch : z, dst);
+      dma_b128(at[i] >= 0 ? (const char *)(vc + at[i]) + 16 * ch : z, dst + Sh::kTileBytes);
+    }
+  };
+
+  // Addresses within a tile, base ^ (chunk << 4) + row * RB: rows that differ by
+  // 16 share their XOR, so a tile's reads have few distinct addresses and the rest
+  // are immediate offsets.
+  const unsigned k_at = c * RB + ((hf ^ swz(c)) << 4);
+  const int vr0 = B16 ? 4 * hf + ((lane & 15) >> 2) : 4 * hf;
+  const unsigned v_at = B16 ? vr0 * RB + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swz(vr0)) << 4) + 8 * (lane & 1)
+                            : vr0 * RB + (((c >> 2) ^ swz(vr0)) << 4) + 4 * (c & 3);
+
+  const int tiles = key_end > key_first ? (key_end - key_first + KT - 1) / KT : 0;
+  if (tid < 4) s_bad[tid] = -1;
+  __syncthreads();
+  if (tiles > 0) {
+    look_up(key_first, 0);
+    copy(0);
+    if (tiles > 1) look_up(key_first + KT, 1);
+  }
+  for (int it = 0; it < tiles; it++) {
+    const int key0 = key_first + it * KT;
+    wait_dma();
+    __syncthreads();
+    if (it + 1 < tiles) {
+      copy((it + 1) & 1);
+      if (it + 2 < tiles) look_up(key0 + 2 * KT, it + 2);
+    }
+    if (key0 > wave_any) continue;
+    const unsigned tile_at = lds0 + (it & 1) * 2 * Sh::kTileBytes;
+    // formed anew for each tile: kept over the loop, they would fill the registers
+    unsigned ka = k_at + tile_at, va = v_at + tile_at + Sh::kTileBytes;
+    asm volatile("" : "+v"(ka), "+v"(va));
+    v16f sc[NS];
+#pragma unroll
+    for (int b = 0; b < NS; b++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) sc[b][i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KC; i++)
+#pragma unroll
+      for (int b = 0; b < NS; b++) {
+        const v4u kf = lds_v4u((ka ^ (i << 5)) + 32 * b * RB);
+        if constexpr (B16) {
+          sc[b] = Mat16<T>::mul32(kf, qv[i], sc[b]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) sc[b] = mfma_f32_32(__uint_as_float(kf[e]), __uint_as_float(qv[i][e]), sc[b]);
+          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    // register i of subtile b: position key0 + 32 b + 8 (i / 4) + 4 hf + i % 4
+    const bool bad = s_bad[it & 3] == it;
+    if (key0 + KT - 1 > wave_all || key0 + KT > key_end || bad) {
+#pragma unroll
+      for (int b = 0; b < NS; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int p = key0 + 32 * b + 8 * (i / 4) + 4 * hf + i % 4;
+          bool see = p <= lim && p < key_end;
+          if (bad && see) see = cell(a.map, tab, p) >= 0;
+          sc[b][i] = see ? sc[b][i] * a.scale : -INFINITY;
+        }
+    } else {
+#pragma unroll
+      for (int b = 0; b < NS; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) sc[b][i] *= a.scale;
+    }
+    float bm = sc[0][0];
+#pragma unroll
+    for (int b = 0; b < NS; b++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[b][i]);
+    bm = fmaxf(bm, __shfl_xor(bm, 32));
+    const float m_new = fmaxf(m_run, bm), m_use = m_new == -INFINITY ? 0.0f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+    float ps = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NS; b++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        sc[b][i] = __builtin_amdgcn_exp2f(sc[b][i] - m_use);
+        ps += sc[b][i];
+      }
+    ps += __shfl_xor(ps, 32);
+    l_run = __builtin_fmaf(l_run, alpha, ps);
+    if (__any(m_new != m_run)) {
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] *= alpha;
+    }
+    m_run = m_new;
+    if constexpr (B16) {
+      constexpr int swz8 = CPR == 8 ? 4 : 8;  // swz of a row 8 further
+#pragma unroll
+      for (int st = 0; st < KT / 16; st++) {
+        const int b = st / 2, g = 8 * (st % 2);
+        const v4u pf = v4u{pack2<T>(sc[b][g], sc[b][g + 1]), pack2<T>(sc[b][g + 2], sc[b][g + 3]),
+                           pack2<T>(sc[b][g + 4], sc[b][g + 5]), pack2<T>(sc[b][g + 6], sc[b][g + 7])};
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          v2u vf[2];
+#pragma unroll
+          for (int q = 0; q < 2; q++)
+            vf[q] = lds_transposed((va ^ (d << 6) ^ (q * swz8 << 4)) + (16 * st + 8 * q) * RB);
+          o[d] = Mat16<T>::mul32(v4u{vf[0][0], vf[0][1], vf[1][0], vf[1][1]}, pf, o[d]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int r = 8 * (i / 4) + i % 4;
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          const float vf = lds_f32((va ^ (((8 * d) ^ (r & 15)) << 4)) + r * RB);
+          o[d] = mfma_f32_32(vf, sc[0][i], o[d]);
+        }
+        if (i % 2) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  if (!live) return;
+  if (a.po) {
+    const size_t rec = ((size_t)split * a.rows + (a.start[s] - a.start[0] + tok)) * a.nh + head;
+    if (hf == 0) {
+      a.pm[rec] = m_run;
+      a.pl[rec] = l_run;
+    }
+    if (m_run == -INFINITY) return;
+    float *po = a.po + rec * HD;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        *(v4f *)(po + 32 * d + 8 * i + 4 * hf) = v4f{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+    return;
+  }
+  const float inv = l_run > 0.0f ? 1.0f / l_run : l_run == 0.0f ? 0.0f : l_run;
+  const T *gp = a.gate ? (const T *)a.gate + (size_t)(a.start[s] + tok) * a.gate_stride + (size_t)head * a.gate_head : nullptr;
+  T *op = (T *)a.out + qrow * HD;
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int dim = 32 * d + 8 * i + 4 * hf;
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = o[d][4 * i + e] * inv;
+      if (gp) {
+        const Pack<T, 4> g = *(const Pack<T, 4> *)(gp + dim);
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] *= gate_sigmoid((float)g.v[e]);
+      }
+      Pack<T, 4> r;
+#pragma unroll
+      for (int e = 0; e < 4; e++) r.v[e] = (T)y[e];
+      *(Pack<T, 4> *)(op + dim) = r;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+bool pools_ok(const char *name, const ColiPaged *c, const void *k_pool, const void *v_pool, const int *table) {
+  if (!c) return fail_arg("%s: null cache description", name), false;
+  if (!type_bytes(c->type)) return fail_arg("%s: unknown element type %d", name, c->type), false;
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail_arg("%s: head_dim %d is not 64, 128 or 256", name, c->head_dim), false;
+  if (c->kv_heads <= 0 || c->query_heads <= 0 || c->query_heads % c->kv_heads || c->query_heads > 65535)
+    return fail_arg("%s: query_heads %d (1..65535) must be a multiple of kv_heads %d", name, c->query_heads, c->kv_heads),
+           false;
+  if (c->page_size <= 0 || c->pages <= 0 || c->table_pages <= 0 || (long long)c->pages * c->page_size > INT_MAX ||
+      (long long)c->table_pages * c->page_size > INT_MAX)
+    return fail_arg("%s: page_size, pages and table_pages must be positive, their products below 2^31", name), false;
+  const long long page = (long long)c->page_size * c->kv_heads * c->head_dim;
+  if (c->page_stride < page || c->page_stride % 8 || c->page_stride > LLONG_MAX / 8 / c->pages)
+    return fail_arg("%s: page_stride %lld must be a multiple of 8 and at least one page's %lld elements", name,
+                    c->page_stride, page),
+           false;
+  if (!k_pool || !v_pool || !table) return fail_arg("%s: null pool or page table", name), false;
+  if (!aligned16(k_pool) || !aligned16(v_pool)) return fail_arg("%s: pools must be 16-byte aligned", name), false;
+  if ((uintptr_t)table & 3) return fail_arg("%s: the page table must be 4-byte aligned", name), false;
+  return true;
+}
+
+bool rows_ok(const char *name, const ColiPaged *c, const int *start, const int *length, int sequences) {
+  if (sequences < 0 || (sequences && !length)) return fail_arg("%s: null lengths or negative sequence count", name), false;
+  if (start && sequences && start[0] < 0) return fail_arg("%s: start[0] is negative", name), false;
+  for (int s = 0; s < sequences; s++) {
+    if (length[s] < 0 || length[s] > (long long)c->table_pages * c->page_size)
+      return fail_arg("%s: length[%d] = %d is outside 0..%lld", name, s, length[s], (long long)c->table_pages * c->page_size),
+             false;
+    if (start && (start[s + 1] < start[s] || start[s + 1] - start[s] > length[s]))
+      return fail_arg("%s: sequence %d has rows %d..%d and length %d", name, s, start[s], start[s + 1], length[s]), false;
+  }
+  return true;
+}
+
+bool gate_ok(const char *name, const ColiPaged *c, const void *gate, long long stride, int head) {
+  if (!gate) return true;
+  if (((uintptr_t)gate & (4 * type_bytes(c->type) - 1)) || stride % 4 || head % 4 || stride < 0 || head < 0)
+    return fail_arg("%s: gates must be aligned to four elements, their strides non-negative multiples of 4", name), false;
+  return true;
+}
+
+PageMap page_map(const ColiPaged *c, const int *table) {
+  return {table, c->pages, c->table_pages, c->page_size, fast_div(c->page_size), c->page_stride, c->kv_heads * c->head_dim};
+}
+
+int cus_of(const ColiCuda *ctx) { return ctx->sm_count > 0 ? ctx->sm_count : 256; }
+
+template <class T>
+void launch_append(const AppendArgs &a, int hd, dim3 grid, hipStream_t st) {
+  if (hd == 64)
+    k_paged_append<T, 64><<<grid, 256, 0, st>>>(a);
+  else if (hd == 128)
+    k_paged_append<T, 128><<<grid, 256, 0, st>>>(a);
+  else
+    k_paged_append<T, 256><<<grid, 256, 0, st>>>(a);
+}
+
+template <class T, int HD>
+void launch_decode(const DecodeArgs &a, unsigned grid, hipStream_t st) {
+  if (a.map.page_size % 16 == 0)
+    k_paged_decode<T, HD, true><<<grid, 256, 0, st>>>(a);
+  else
+    k_paged_decode<T, HD, false><<<grid, 256, 0, st>>>(a);
+}
+template <class T>
+void launch_decode(const DecodeArgs &a, int hd, unsigned grid, hipStream_t st) {
+  if (hd == 64)
+    launch_decode<T, 64>(a, grid, st);
+  else if (hd == 128)
+    launch_decode<T, 128>(a, grid, st);
+  else
+    launch_decode<T, 256>(a, grid, st);
+}
+
+template <class T>
+void launch_join(const JoinArgs &a, int hd, int rows, hipStream_t st) {
+  for (int r0 = 0; r0 < rows; r0 += 65535) {  // only rows of one split count (not flat) pass this limit
+    JoinArgs b = a;
+    const int n = rows - r0 < 65535 ? rows - r0 : 65535;
+    b.row0 += r0;
+    b.po += (size_t)r0 * a.nh * hd;
+    b.pm += (size_t)r0 * a.nh;
+    b.pl += (size_t)r0 * a.nh;
+    const dim3 grid(a.nh, n);
+    if (hd == 64)
+      k_paged_join<T, 64><<<grid, 256, 0, st>>>(b);
+    else if (hd == 128)
+      k_paged_join<T, 128><<<grid, 256, 0, st>>>(b);
+    else
+      k_paged_join<T, 256><<<grid, 256, 0, st>>>(b);
+  }
+}
+
+constexpr int kPromptRows = 128;
+template <class T, int HD>
+int launch_prompt(const char *name, const PromptArgs &a, dim3 grid, hipStream_t st) {
+  typedef PromptShape<T, HD> Sh;
+  const hipError_t e =
+      hipFuncSetAttribute((const void *)k_paged_prompt<T, HD>, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds);
+  if (e != hipSuccess) return fail_hip(name, e);
+  k_paged_prompt<T, HD><<<grid, 64 * Sh::kWaves, Sh::kLds, st>>>(a);
+  return 0;
+}
+static_assert(PromptShape<float, 64>::kRows == kPromptRows && PromptShape<__bf16, 256>::kRows == kPromptRows, "rows of a tile");
+template <class T>
+int launch_prompt(const char *name, const PromptArgs &a, int hd, dim3 grid, hipStream_t st) {
+  return hd == 64 ? launch_prompt<T, 64>(name, a, grid, st)
+                  : hd == 128 ? launch_prompt<T, 128>(name, a, grid, st) : launch_prompt<T, 256>(name, a, grid, st);
+}
+int prompt_keys(int type) { return type != COLI_TYPE_F32 ? 64 : 32; }
+
+// Partial records of n (split, row) pairs: outputs, maxima, sums.
+int partials(ColiCuda *ctx, const char *name, size_t n, int nh, int hd, float **po, float **pm, float **pl) {
+  const size_t heads = n * nh;
+  if (ensure_scratch(ctx, kScrPaged, heads * (hd + 2) * sizeof(float), name)) return -1;
+  *po = (float *)ctx->scratch[kScrPaged];
+  *pm = *po + heads * hd;
+  *pl = *pm + heads;
+  return 0;
+}
+
+}  // namespace
+}  // namespace sw
+
+using namespace sw;
+
+extern "C" int coli_cuda_paged_append(ColiCuda *ctx, const ColiPaged *c, void *k_pool, void *v_pool, const int *table,
+                                      const int *start, const int *length, int sequences, void *q_out, const void *q,
+                                      long long q_stride, int q_head_stride, const void *k, long long k_stride,
+                                      const void *v, long long v_stride, const float *q_norm, const float *k_norm,
+                                      float eps, int rotary_dim, float theta) {
+  static const char *name = "coli_cuda_paged_append";
+  if (!pools_ok(name, c, k_pool, v_pool, table)) return -1;
+  if (sequences && !start) return fail_arg("%s: null start", name);
+  if (!rows_ok(name, c, start, length, sequences)) return -1;
+  if (!k || !v || !q != !q_out) return fail_arg("%s: null keys or values, or one of q and q_out", name);
+  if (!aligned16(k) || !aligned16(v) || !aligned16(q) || !aligned16(q_out) || k_stride % 8 || v_stride % 8 ||
+      (q && (q_stride % 8 || q_head_stride % 8)) || k_stride < 0 || v_stride < 0 || q_stride < 0 || q_head_stride < 0)
+    return fail_arg("%s: tensors must be 16-byte aligned, strides non-negative multiples of 8 elements", name);
+  if (((uintptr_t)q_norm | (uintptr_t)k_norm) & 3) return fail_arg("%s: norms must be 4-byte aligned", name);
+  if (rotary_dim < 0 || rotary_dim > c->head_dim || rotary_dim % 2)
+    return fail_arg("%s: rotary_dim %d must be even and within head_dim", name, rotary_dim);
+  if (rotary_dim && !(theta > 0.0f && theta < INFINITY)) return fail_arg("%s: theta must be positive and finite", name);
+  if ((q_norm || k_norm) && !(eps >= 0.0f && eps < INFINITY)) return fail_arg("%s: eps must be finite, not negative", name);
+  if (!ctx) return fail_arg("%s: null context", name);
+  OnDevice on(ctx);
+  AppendArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = q, a.k = k, a.v = v;
+  a.q_out = q_out, a.k_pool = k_pool, a.v_pool = v_pool;
+  a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
+  a.q_norm = q_norm, a.k_norm = k_norm;
+  a.q_head = q_head_stride, a.nh = c->query_heads, a.nkv = c->kv_heads, a.rd = rotary_dim;
+  a.eps = eps;
+  a.map = page_map(c, table);
+  if (rotary_dim) {
+    // theta^(-2 i / rotary_dim) / 2 pi by repeated products in 64 bits (127 of them: 2^-46)
+    const double ratio = pow((double)theta, -2.0 / rotary_dim);
+    a.freq[0] = 0.15915494309189535;
+    for (int i = 1; i < rotary_dim / 2; i++) a.freq[i] = a.freq[i - 1] * ratio;
+  }
+  const int heads = (q ? c->query_heads : 0) + c->kv_heads;
+  for (int s0 = 0; s0 < sequences; s0 += kSeqs) {
+    const int n = sequences - s0 < kSeqs ? sequences - s0 : kSeqs, rows = start[s0 + n] - start[s0];
+    if (!rows) continue;
+    memcpy(a.start, start + s0, (n + 1) * sizeof(int));
+    memcpy(a.len, length + s0, n * sizeof(int));
+    a.seqs = n;
+    a.first_seq = s0;
+    // few tokens: their heads over several workgroups, four heads (one a wave) at least
+    int gy = 4 * cus_of(ctx) / rows;
+    if (gy > (heads + 3) / 4) gy = (heads + 3) / 4;
+    if (gy < 1) gy = 1;
+    a.heads_per_block = ((heads + gy - 1) / gy + 3) / 4 * 4;
+    const dim3 grid(rows, (heads + a.heads_per_block - 1) / a.heads_per_block);
+    if (c->type == COLI_TYPE_F32)
+      launch_append<float>(a, c->head_dim, grid, ctx->stream);
+    else if (c->type == COLI_TYPE_F16)
+      launch_append<_Float16>(a, c->head_dim, grid, ctx->stream);
+    else
+      launch_append<__bf16>(a, c->head_dim, grid, ctx->stream);
+  }
+  return launch_status(name);
+}
+
+extern "C" int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *c, void *out, const void *q, const void *gate,
+                                      long long gate_stride, int gate_head_stride, const void *k_pool, const void *v_pool,
+                                      const int *table, const int *length, int sequences, float scale) {
+  static const char *name = "coli_cuda_paged_decode";
+  if (!pools_ok(name, c, k_pool, v_pool, table) || !rows_ok(name, c, nullptr, length, sequences) ||
+      !gate_ok(name, c, gate, gate_stride, gate_head_stride))
+    return -1;
+  if (!out || !q || !aligned16(out) || !aligned16(q)) return fail_arg("%s: q and out must be 16-byte aligned", name);
+  if (!isfinite(scale)) return fail_arg("%s: scale is not finite", name);
+  if (!ctx) return fail_arg("%s: null context", name);
+  OnDevice on(ctx);
+  const int nh = c->query_heads, hd = c->head_dim, size = type_bytes(c->type);
+  DecodeArgs a;
+  memset(&a, 0, sizeof(a));
+  a.k = k_pool, a.v = v_pool;
+  a.gate_stride = gate_stride;
+  a.gate_head = gate_head_stride;
+  a.nh = nh, a.nkv = c->kv_heads, a.G = nh / c->kv_heads;
+  a.hgroups = (a.G + 15) / 16;
+  a.scale = scale * kLog2e;
+  a.map = page_map(c, table);
+  const long long items = (long long)c->kv_heads * a.hgroups;
+  const int least = c->type == COLI_TYPE_F32 ? 64 : 128;  // one block a wave
+  for (int s0 = 0; s0 < sequences; s0 += kSeqs) {
+    const int n = sequences - s0 < kSeqs ? sequences - s0 : kSeqs;
+    long long total = 0;
+    int longest = 0;
+    for (int r = 0; r < n; r++) {
+      total += length[s0 + r];
+      if (length[s0 + r] > longest) longest = length[s0 + r];
+    }
+    // all splits of one length, two workgroups a compute unit in all
+    long long per = (total * items + 2 * cus_of(ctx) - 1) / (2 * cus_of(ctx));
+    if (per < (longest + kMaxSplits - 1) / kMaxSplits) per = (longest + kMaxSplits - 1) / kMaxSplits;
+    per = (per + least - 1) / least * least;
+    if (per < least) per = least;
+    a.per = per < INT_MAX / 2 ? (int)per : INT_MAX / 2 / least * least;
+    bool one = true;
+    a.first[0] = 0;
+    for (int r = 0; r < n; r++) {
+      const int S = length[s0 + r] <= a.per ? 1 : (int)(((long long)length[s0 + r] + a.per - 1) / a.per);
+      a.first[r + 1] = a.first[r] + S;
+      one = one && S == 1;
+    }
+    memcpy(a.len, length + s0, n * sizeof(int));
+    a.rows = n;
+    a.first_seq = s0;
+    a.q = (const char *)q + (size_t)s0 * nh * hd * size;
+    a.out = (char *)out + (size_t)s0 * nh * hd * size;
+    a.gate = gate ? (const char *)gate + (size_t)s0 * gate_stride * size : nullptr;
+    a.po = a.pm = a.pl = nullptr;
+    if (!one && partials(ctx, name, a.first[n], nh, hd, &a.po, &a.pm, &a.pl)) return -1;
+    const unsigned grid = (unsigned)(a.first[n] * items);
+    if (c->type == COLI_TYPE_F32)
+      launch_decode<float>(a, hd, grid, ctx->stream);
+    else if (c->type == COLI_TYPE_F16)
+      launch_decode<_Float16>(a, hd, grid, ctx->stream);
+    else
+      launch_decode<__bf16>(a, hd, grid, ctx->stream);
+    if (one) continue;
+    JoinArgs j;
+    memset(&j, 0, sizeof(j));
+    j.po = a.po, j.pm = a.pm, j.pl = a.pl;
+    j.gate = a.gate;
+    j.out = a.out;
+    j.gate_stride = gate_stride;
+    j.gate_head = gate_head_stride;
+    j.nh = nh;
+    j.flat = 1;
+    memcpy(j.first, a.first, sizeof(a.first));
+    if (c->type == COLI_TYPE_F32)
+      launch_join<float>(j, hd, n, ctx->stream);
+    else if (c->type == COLI_TYPE_F16)
+      launch_join<_Float16>(j, hd, n, ctx->stream);
+    else
+      launch_join<__bf16>(j, hd, n, ctx->stream);
+  }
+  return launch_status(name);
+}
+
+extern "C" int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *c, void *out, const void *q, const void *gate,
+                                      long long gate_stride, int gate_head_stride, const void *k_pool, const void *v_pool,
+                                      const int *table, const int *start, const int *length, int sequences, float scale) {
+  static const char *name = "coli_cuda_paged_prompt";
+  if (!pools_ok(name, c, k_pool, v_pool, table)) return -1;
+  if (sequences && !start) return fail_arg("%s: null start", name);
+  if (!rows_ok(name, c, start, length, sequences) || !gate_ok(name, c, gate, gate_stride, gate_head_stride)) return -1;
+  if (!out || !q || !aligned16(out) || !aligned16(q)) return fail_arg("%s: q and out must be 16-byte aligned", name);
+  if (!isfinite(scale)) return fail_arg("%s: scale is not finite", name);
+  const int nh = c->query_heads, hd = c->head_dim, G = nh / c->kv_heads, R = kPromptRows;
+  for (int s = 0; s < sequences; s++)
+    if ((long long)(start[s + 1] - start[s]) * G > INT_MAX - R)
+      return fail_arg("%s: sequence %d has %d rows of %d heads a kv head: more than 2^31", name, s, start[s + 1] - start[s], G);
+  if (!ctx) return fail_arg("%s: null context", name);
+  OnDevice on(ctx);
+  PromptArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = q, a.k = k_pool, a.v = v_pool;
+  a.out = out;
+  a.gate = gate;
+  a.gate_stride = gate_stride;
+  a.gate_head = gate_head_stride;
+  a.nh = nh, a.nkv = c->kv_heads, a.G = G;
+  a.scale = scale * kLog2e;
+  a.by_group = fast_div(G);
+  a.map = page_map(c, table);
+  for (int s0 = 0; s0 < sequences; s0 += kSeqs) {
+    const int n = sequences - s0 < kSeqs ? sequences - s0 : kSeqs, rows = start[s0 + n] - start[s0];
+    if (!rows) continue;
+    long long tiles = 0;
+    int longest = 0;
+    a.tile0[0] = 0;
+    for (int s = 0; s < n; s++) {
+      const int m = start[s0 + s + 1] - start[s0 + s];
+      tiles += ((long long)m * G + R - 1) / R;
+      if (tiles > INT_MAX) return fail_arg("%s: too many rows", name);
+      a.tile0[s + 1] = (int)tiles;
+      if (m && length[s0 + s] > longest) longest = length[s0 + s];
+    }
+    memcpy(a.start, start + s0, (n + 1) * sizeof(int));
+    memcpy(a.len, length + s0, n * sizeof(int));
+    a.seqs = n;
+    a.first_seq = s0;
+    a.rows = rows;
+    // few tiles: their positions over several workgroups, four tiles of positions each at least
+    long long splits = cus_of(ctx) / (tiles * c->kv_heads), most = longest / (4 * prompt_keys(c->type));
+    if (splits > most) splits = most;
+    if (splits > kMaxSplits) splits = kMaxSplits;
+    a.splits = splits < 1 ? 1 : (int)splits;
+    a.po = a.pm = a.pl = nullptr;
+    if (a.splits > 1 && partials(ctx, name, (size_t)a.splits * rows, nh, hd, &a.po, &a.pm, &a.pl)) return -1;
+    const dim3 grid((unsigned)tiles, c->kv_heads, a.splits);
+    const int rc = c->type == COLI_TYPE_F32   ? launch_prompt<float>(name, a, hd, grid, ctx->stream)
+                   : c->type == COLI_TYPE_F16 ? launch_prompt<_Float16>(name, a, hd, grid, ctx->stream)
+                                              : launch_prompt<__bf16>(name, a, hd, grid, ctx->stream);
+    if (rc) return -1;
+    if (a.splits == 1) continue;
+    JoinArgs j;
+    memset(&j, 0, sizeof(j));
+    j.po = a.po, j.pm = a.pm, j.pl = a.pl;
+    j.gate = gate;
+    j.out = out;
+    j.gate_stride = gate_stride;
+    j.gate_head = gate_head_stride;
+    j.nh = nh;
+    j.S = a.splits;
+    j.step = rows;
+    j.row0 = start[s0];
+    if (c->type == COLI_TYPE_F32)
+      launch_join<float>(j, hd, rows, ctx->stream);
+    else if (c->type == COLI_TYPE_F16)
+      launch_join<_Float16>(j, hd, rows, ctx->stream);
+    else
+      launch_join<__bf16>(j, hd, rows, ctx->stream);
+  }
+  return launch_status(name);
+}

@@ -41,6 +41,7 @@ enum Scratch {
   kScrBlock,       // MoE block: normalised activations and the MoE output
   kScrHead,        // output head: quantised normalised rows and their scales
   kScrMixer,       // Gated DeltaNet / GQA layers: staged inputs, projections, partials
+  kScrPaged,       // paged attention: partial records of splits
   kScrCount
 };
 
