@@ -629,6 +629,45 @@ int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *cache, void *out,
                            const int *table, const int *start,
                            const int *length, int sequences, float scale);
 
+/* The gated delta rule of the Gated DeltaNet layer, between its convolution and
+ * its output norm, with the layer's gates: for every token of a sequence in order
+ *   S <- e^g S;  d = beta (v - S^T k);  S <- S + k d^T;  out = S^T q
+ * a value head, with q and k of its key head (value_heads / key_heads value heads
+ * each) divided by sqrt(sum of squares + 1e-6), q by sqrt(key_dim) too,
+ * g = -exp(a_log[head]) softplus(a + dt_bias[head]) and beta = sigmoid(b).
+ * q, k [rows][key_heads][key_dim], v [rows][value_heads][value_dim] of the
+ * element type, strides in elements from row to row, heads contiguous (the rows
+ * of the convolution, q | k | v, do as they are); a, b [rows][value_heads], a_log,
+ * dt_bias [value_heads] fp32; out [rows][value_heads][value_dim] contiguous, of
+ * the element type, overlapping no input.  States are [slots][value_heads]
+ * [key_dim][value_dim] fp32, those of coli_cuda_gdn_*: a sequence's is read from
+ * its slot of `state` and left in the same slot of `state_out`, which is `state`
+ * itself or apart from it.  A call names a slot once.
+ *
+ * key_dim a multiple of 8 up to 128, value_dim of 32 up to 256; tensors 16-byte
+ * aligned, strides multiples of 8. */
+typedef struct {
+  int type; /* COLI_TYPE_*: q, k, v, out */
+  int key_heads, value_heads, key_dim, value_dim, slots;
+  long long q_stride, k_stride, v_stride;
+} ColiDelta;
+/* One token of each of `rows` sequences, row r in slot[r] (host array). */
+int coli_cuda_delta_step(ColiCuda *ctx, const ColiDelta *d, void *out,
+                         const void *q, const void *k, const void *v,
+                         const float *a, const float *b, const float *a_log,
+                         const float *dt_bias, const float *state,
+                         float *state_out, const int *slot, int rows);
+/* Packed prompts: sequence s is rows start[s] .. start[s + 1] - 1 and continues
+ * slot[s] (host arrays; start ascending from start[0] >= 0, sequences + 1
+ * entries).  A sequence without rows keeps its state.  Rows of no sequence are
+ * neither read nor written. */
+int coli_cuda_delta_prompt(ColiCuda *ctx, const ColiDelta *d, void *out,
+                           const void *q, const void *k, const void *v,
+                           const float *a, const float *b, const float *a_log,
+                           const float *dt_bias, const float *state,
+                           float *state_out, const int *start,
+                           const int *slot, int sequences);
+
 #ifdef __cplusplus
 }
 #endif

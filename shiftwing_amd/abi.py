@@ -29,6 +29,12 @@ class ColiPaged(C.Structure):
                 ("page_size", C.c_int), ("pages", C.c_int), ("table_pages", C.c_int), ("page_stride", C.c_longlong)]
 
 
+class ColiDelta(C.Structure):
+    _fields_ = [("type", C.c_int), ("key_heads", C.c_int), ("value_heads", C.c_int), ("key_dim", C.c_int),
+                ("value_dim", C.c_int), ("slots", C.c_int), ("q_stride", C.c_longlong), ("k_stride", C.c_longlong),
+                ("v_stride", C.c_longlong)]
+
+
 _SCALARS = {
     "int": C.c_int, "float": C.c_float, "size_t": C.c_size_t, "void": None,
     "unsigned long long": C.c_ulonglong, "long long": C.c_longlong, "double": C.c_double,

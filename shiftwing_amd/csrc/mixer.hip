@@ -437,10 +437,6 @@ struct GdnArgs {
   GdnGroups grp;
 };
 
-__device__ __forceinline__ float softplus_ref(float x) {
-  return x > 20.f ? x : (x < -20.f ? expf(x) : log1pf(expf(x)));
-}
-
 __global__ __launch_bounds__(64) void k_gdn_recur(GdnArgs g) {
   const int nsp = (g.dv + 31) / 32;
   const int h = blockIdx.x / nsp, js = blockIdx.x % nsp, gi = blockIdx.y;

@@ -42,6 +42,7 @@ enum Scratch {
   kScrHead,        // output head: quantised normalised rows and their scales
   kScrMixer,       // Gated DeltaNet / GQA layers: staged inputs, projections, partials
   kScrPaged,       // paged attention: partial records of splits
+  kScrDelta,       // packed Gated DeltaNet: per-chunk records
   kScrCount
 };
 

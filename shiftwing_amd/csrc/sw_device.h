@@ -82,6 +82,11 @@ __device__ __forceinline__ float sigmoid_ref(float x) { return sigmoid_ref_t(x, 
 __device__ __forceinline__ float silu_ref_t(float x, const uint64_t *tab) { return x * sigmoid_ref_t(x, tab); }
 __device__ __forceinline__ float silu_ref(float x) { return x * sigmoid_ref(x); }
 
+// softplus of the Gated DeltaNet's decay (c/qwen.c:2907-2927)
+__device__ __forceinline__ float softplus_ref(float x) {
+  return x > 20.f ? x : (x < -20.f ? expf(x) : log1pf(expf(x)));
+}
+
 // ---------------------------------------------------------------------------
 // wave64 reductions
 // ---------------------------------------------------------------------------
