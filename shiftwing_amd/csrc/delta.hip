@@ -16,7 +16,7 @@
 // for all chunks at once (k_delta_chunk), the rest walks a sequence's chunks
 // (k_delta_scan).  Every exponent is a sum of g over tokens s+1 .. t, never positive,
 // taken as a difference of 64-bit running sums, which keeps it however far G has run.
-// All products are fp32.
+// All products are fp32, or bf16 parts that make up fp32 (kTri below).
 #include <hip/hip_runtime.h>
 #include <limits.h>
 #include <stdlib.h>
@@ -30,11 +30,20 @@ namespace {
 constexpr int kChunk = 64;
 constexpr int kKey = 128;   // largest key_dim
 constexpr int kSlice = 32;  // value columns of a k_delta_scan workgroup
-// one (chunk, value head) record of k_delta_chunk, in floats: the inverse and P, row
-// by row, then per token e^G |k|^-1, e^G |q|^-1 key_dim^-1/2 and e^(G_63 - G) |k|^-1,
-// then e^G_63
-constexpr int kRecInv = 0, kRecP = kChunk * kChunk, kRecX = 2 * kChunk * kChunk, kRecQ = kRecX + kChunk,
-              kRecR = kRecQ + kChunk, kRecEnd = kRecR + kChunk, kRec = kRecEnd + kChunk;
+
+// fp32 values as sums of three bf16 ones: 8 bits each, the rest exactly 24 (a bf16
+// value is one of them, an fp16 value two).  Products of such sums on the bf16 matrix
+// cores, without the terms below 2^-24, are fp32 products in all but rounding, at 3
+// (one factor bf16) to 6 instructions of 16 cycles where the fp32 matrix cores take 8
+// of 32 for the same tile.
+constexpr int kTri = 10 * 256;  // elements of a 64 x 64 lower triangle in 16 x 16 tiles
+// One (chunk, value head) record of k_delta_chunk: the inverse of 1 + A times beta, and
+// P, as three bf16 triangles each; then per token e^G |k|^-1, e^G |q|^-1 key_dim^-1/2
+// and e^(G_63 - G) |k|^-1, then e^G_63, in fp32.  A triangle's row tile i is
+// [16 rows][16 (i + 1)] at 128 i (i + 1), which gives a lane its matrix operand in one load.
+constexpr int kRecInv = 0, kRecP = 3 * kTri * 2, kRecX = 2 * kRecP, kRecQ = kRecX + kChunk * 4,
+              kRecR = kRecQ + kChunk * 4, kRecEnd = kRecR + kChunk * 4, kRec = kRecEnd + 16;  // bytes
+static_assert(kRec % 16 == 0, "records are 16-byte aligned");
 
 struct DeltaArgs {
   const void *q, *k, *v;
@@ -42,14 +51,36 @@ struct DeltaArgs {
   const float *a, *b, *a_log, *dt_bias;
   const float *state;
   float *state_out;
-  float *rec;
+  char *rec;
   long long q_stride, k_stride, v_stride;
   int kh, vh, dk, dv, seqs;
-  int chunk_first;           // k_delta_chunk / k_delta_scan: first chunk of each sequence in this pass
-  int chunks;                // chunks of a sequence in one pass, at most
-  int start[kSeqs + 1], slot[kSeqs];
-  int chunk0[kSeqs + 1];     // records of sequence s: chunk0[s] .. chunk0[s + 1] - 1
+  int chunk_first;  // first chunk of each sequence in this pass
+  int chunks;       // chunks of a sequence in one pass, at most
+  int begin[kSeqs], rows[kSeqs], slot[kSeqs];
+  int chunk0[kSeqs + 1];  // records of sequence s: chunk0[s] .. chunk0[s + 1] - 1
 };
+
+// x as three bf16 values, packed two by two
+__device__ __forceinline__ void split3(const float (&x)[4], v2u (&p)[3]) {
+  float r[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) r[e] = x[e];
+#pragma unroll
+  for (int k = 0; k < 3; k++) {
+    __bf16 h[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      h[e] = (__bf16)r[e];
+      r[e] -= (float)h[e];
+    }
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    p[k] = v2u{__builtin_bit_cast(unsigned, v2b{h[0], h[1]}), __builtin_bit_cast(unsigned, v2b{h[2], h[3]})};
+  }
+}
+template <class T>
+constexpr int planes_of() {
+  return sizeof(T) == 4 ? 3 : __is_same(T, __bf16) ? 1 : 2;
+}
 
 // Eight elements from 16-byte aligned memory.
 template <class T>
@@ -170,254 +201,455 @@ __global__ __launch_bounds__(256) void k_delta_step(StepArgs g) {
 __device__ __forceinline__ v4f mfma_f32_16(float a, float b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ v4f mfma_b16(v4u a, v4u b, v4f c) { return Mat16<__bf16>::mul16(a, b, c); }
+constexpr int kPitchB = kKey * 2 + 16;  // bytes of a 16-bit row in LDS: 16 rows' pieces lie in distinct banks
+constexpr int kPitchF = kKey * 4 + 16;  // of an fp32 row
 
-// A chunk's raw rows of one key head as fp32, [token][kPitch], zero beyond the
-// sequence's end and beyond key_dim, and (sq, sk not null) the inverse lengths.
-constexpr int kPitch = kKey + 4;
+// One workgroup a (chunk, key head).  The products of the chunk's keys with its keys
+// and queries, as raw rows (their lengths divide the results), serve every value head
+// of the key head: 10 lower tiles each, formed as K Q^T, so that a lane of the result
+// holds four consecutive columns s of one row t.  Then a wave takes a value head:
+// gates (token a lane) and their running sum, A and P tile by tile, the inverse:
+// its four 16 x 16 diagonal tiles by substitution, all at once (lane = tile and
+// column), the others from
+//   T_ij = -(sum_{j < k <= i} T_ik A_kj) T_jj
+// in transposed form on the fp32 matrix cores, where a result's registers are the next
+// product's B operand as they stand.
+// e^(G_t - G_s) off the diagonal tiles is e^(G_t - R) e^(R - G_s), R the sum at the end
+// of s's tile: both exponents are negative, and a tile takes two factors a lane.
+struct ChunkLds {
+  static constexpr int kPairs = 0;                       // tiles of k k^T, then q k^T: [tile][lane] x 16 bytes
+  static constexpr int kNorms = kPairs + 20 * 1024;      // |k|^-1, |q|^-1 key_dim^-1/2
+  static constexpr int kWork = kNorms + 2 * kChunk * 4;  // raw rows, then per wave:
+  static constexpr int kTile = 16 * 20 * 4;              // a 16 x 16 fp32 tile, rows of 80 bytes
+  static constexpr int kWave = 14 * kTile + kChunk * (8 + 4 * 5);  // 10 tiles of A, 4 of the inverse, G, beta, factors
+};
 template <class T>
-__device__ __forceinline__ void stage_rows(float *rows, const T *src, long long stride, int n, int dk, float *inv) {
-  const int t = threadIdx.x >> 2, p = threadIdx.x & 3;
-  float s2 = 0.0f;
-  for (int c = p; c < kKey / 8; c += 4) {
-    float x[8];
-    if (t < n && 8 * c < dk) {
-      load8(x, src + (size_t)t * stride + 8 * c);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = 0.0f;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e++) s2 = __builtin_fmaf(x[e], x[e], s2);
-    *(float4 *)(rows + t * kPitch + 8 * c) = make_float4(x[0], x[1], x[2], x[3]);
-    *(float4 *)(rows + t * kPitch + 8 * c + 4) = make_float4(x[4], x[5], x[6], x[7]);
-  }
-  if (!inv) return;
-  s2 += __shfl_xor(s2, 1);
-  s2 += __shfl_xor(s2, 2);
-  if (p == 0) inv[t] = 1.f / sqrtf(s2 + 1e-6f);
+constexpr int chunk_lds() {
+  constexpr int rows = 2 * kChunk * (sizeof(T) == 4 ? kPitchF : kPitchB), waves = 4 * ChunkLds::kWave;
+  return ChunkLds::kWork + (rows > waves ? rows : waves);
 }
 
-// One workgroup a (chunk, key head).  The products k k^T and q k^T of the chunk (their
-// lower triangles, in 16 x 16 tiles) serve every value head of the key head; then a
-// wave takes a value head: lane t holds token t's gates, their running sum is a scan
-// of the wave, and lane j solves column j of the inverse by forward substitution,
-// x_t = (t == j) - sum_{s < t} A[t][s] x_s, the column in registers and A's row read
-// from LDS by all lanes at once.
-constexpr int kTri = kChunk + 4;  // pitch of the triangles
 template <class T>
 __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
-  extern __shared__ __align__(16) float lds[];
-  float *s_k = lds, *s_q = lds + kChunk * kPitch;                       // raw rows
-  float *s_kk = s_q + kChunk * kPitch, *s_qk = s_kk + kChunk * kTri;    // triangles
-  float *s_kn = s_qk + kChunk * kTri, *s_qn = s_kn + kChunk;
-  float *s_a = lds;                                                     // per wave, over the rows
+  typedef ChunkLds L;
+  constexpr int kPitch = sizeof(T) == 4 ? kPitchF : kPitchB;
+  extern __shared__ __align__(16) char lds[];
+  v4f *s_pair = (v4f *)(lds + L::kPairs);
+  float *s_kn = (float *)(lds + L::kNorms), *s_qn = s_kn + kChunk;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
   const int hk = blockIdx.y;
   const int s = find_span(g.chunk0, g.seqs, blockIdx.x);
-  const int c = blockIdx.x - g.chunk0[s] + g.chunk_first;
-  const int t0 = g.start[s] + c * kChunk, n = min(kChunk, g.start[s + 1] - t0);
-  stage_rows(s_k, (const T *)g.k + (size_t)t0 * g.k_stride + (size_t)hk * g.dk, g.k_stride, n, g.dk, s_kn);
-  stage_rows(s_q, (const T *)g.q + (size_t)t0 * g.q_stride + (size_t)hk * g.dk, g.q_stride, n, g.dk, s_qn);
-  __syncthreads();
-  const float dks = 1.f / sqrtf((float)g.dk);
-  for (int u = wave; u < 20; u += 4) {  // 10 lower tiles of k k^T, 10 of q k^T
-    int v = u < 10 ? u : u - 10, ti = 0;
-    while (v > ti) v -= ++ti;
-    const float *rows = u < 10 ? s_k : s_q;
-    v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < g.dk; i += 16) {
-      const float4 x = *(const float4 *)(rows + (16 * ti + n16) * kPitch + i + 4 * kg);
-      const float4 y = *(const float4 *)(s_k + (16 * v + n16) * kPitch + i + 4 * kg);
-      acc = mfma_f32_16(x.x, y.x, acc);
-      acc = mfma_f32_16(x.y, y.y, acc);
-      acc = mfma_f32_16(x.z, y.z, acc);
-      acc = mfma_f32_16(x.w, y.w, acc);
-    }
-    const float ncol = s_kn[16 * v + n16];
+  const int first = (blockIdx.x - g.chunk0[s] + g.chunk_first) * kChunk;
+  const int t0 = g.begin[s] + first, n = min(kChunk, g.rows[s] - first);
+
+  // raw rows, zero beyond the sequence's end and beyond key_dim
+  {
+    const int t = threadIdx.x >> 2, p = threadIdx.x & 3;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int r = 16 * ti + 4 * kg + i;
-      const float f = u < 10 ? s_kn[r] : s_qn[r] * dks;
-      (u < 10 ? s_kk : s_qk)[r * kTri + 16 * v + n16] = acc[i] * f * ncol;
+    for (int m = 0; m < 2; m++) {
+      const T *src = m ? (const T *)g.q + (size_t)(t0 + t) * g.q_stride + (size_t)hk * g.dk
+                       : (const T *)g.k + (size_t)(t0 + t) * g.k_stride + (size_t)hk * g.dk;
+      char *row = lds + L::kWork + (m * kChunk + t) * kPitch;
+      float s2 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kKey / 32; i++) {
+        const int c = p + 4 * i;
+        constexpr int V = sizeof(T) / 2;  // 16-byte pieces of eight elements
+        v4u x[V];
+#pragma unroll
+        for (int u = 0; u < V; u++) x[u] = t < n && 8 * c < g.dk ? ((const v4u *)(src + 8 * c))[u] : v4u{0, 0, 0, 0};
+        float f[8];
+        load8(f, (const T *)x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) s2 = __builtin_fmaf(f[e], f[e], s2);
+#pragma unroll
+        for (int u = 0; u < V; u++) ((v4u *)(row + 8 * c * sizeof(T)))[u] = x[u];
+      }
+      s2 += __shfl_xor(s2, 1);
+      s2 += __shfl_xor(s2, 2);
+      if (p == 0) (m ? s_qn : s_kn)[t] = 1.f / sqrtf(s2 + 1e-6f) * (m ? 1.f / sqrtf((float)g.dk) : 1.f);
     }
   }
   __syncthreads();
+  for (int u = wave; u < 20; u += 4) {
+    int j = u < 10 ? u : u - 10, i = 0;
+    while (j > i) j -= ++i;
+    const char *ks = lds + L::kWork + (16 * j + n16) * kPitch;
+    const char *qt = lds + L::kWork + ((u < 10 ? 0 : kChunk) + 16 * i + n16) * kPitch;
+    v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
+    if constexpr (sizeof(T) == 2) {
+      for (int d = 0; d < g.dk; d += 32)
+        acc = Mat16<T>::mul16(*(const v4u *)(ks + 2 * d + 16 * kg), *(const v4u *)(qt + 2 * d + 16 * kg), acc);
+    } else {
+      for (int d = 0; d < g.dk; d += 16) {
+        const v4f x = *(const v4f *)(ks + 4 * d + 16 * kg), y = *(const v4f *)(qt + 4 * d + 16 * kg);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc = mfma_f32_16(x[e], y[e], acc);
+      }
+    }
+    // row s = 16 j + 4 kg + e, column t = 16 i + n16
+    const v4f kn = *(const v4f *)(s_kn + 16 * j + 4 * kg);
+    s_pair[u * 64 + lane] = acc * kn * (u < 10 ? s_kn : s_qn)[16 * i + n16];
+  }
+  __syncthreads();
+
   const int rep = g.vh / g.kh;
-  float *A = s_a + wave * kChunk * kChunk;
+  char *mine = lds + L::kWork + wave * L::kWave;
+  float *s_a = (float *)mine, *s_inv = s_a + 10 * 320;  // tiles [row s][t] of A^T, of the diagonal inverses' transposes
+  double *s_G = (double *)(s_inv + 4 * 320);
+  float *s_beta = (float *)(s_G + kChunk), *s_to = s_beta + kChunk, *s_from = s_to + kChunk;  // s_from [3][64]
   for (int w = wave; w < rep; w += 4) {
     const int h = hk * rep + w;
-    float *rec = g.rec + ((size_t)blockIdx.x * g.vh + h) * kRec;
-    const bool there = lane < n;
-    const size_t tok = (size_t)(t0 + (there ? lane : 0)) * g.vh + h;
-    const float gt = there ? log_decay(expf(g.a_log[h]), g.a[tok], g.dt_bias[h]) : 0.0f;
-    const float beta = there ? sigmoid_ref(g.b[tok]) : 0.0f;
-    const double G = wave_incl_scan_dpp((double)gt);
-    const double Gend = readlane_d63(G);
-    rec[kRecX + lane] = expf((float)G) * s_kn[lane];
-    rec[kRecQ + lane] = expf((float)G) * s_qn[lane] * dks;
-    rec[kRecR + lane] = expf((float)(Gend - G)) * s_kn[lane];
-    if (lane == 0) rec[kRecEnd] = expf((float)Gend);
-    for (int t = 0; t < kChunk; t++) {
-      const int lo = __builtin_amdgcn_readlane(__double2loint(G), t), hi = __builtin_amdgcn_readlane(__double2hiint(G), t);
-      const float bt = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, beta), t));
-      const float e = lane <= t ? expf((float)(__hiloint2double(hi, lo) - G)) : 0.0f;
-      A[t * kChunk + lane] = lane < t ? bt * e * s_kk[t * kTri + lane] : 0.0f;
-      rec[kRecP + t * kChunk + lane] = lane <= t ? e * s_qk[t * kTri + lane] : 0.0f;
+    char *rec = g.rec + ((size_t)blockIdx.x * g.vh + h) * kRec;
+    {
+      const bool there = lane < n;
+      const size_t tok = (size_t)(t0 + (there ? lane : 0)) * g.vh + h;
+      const float gt = there ? log_decay(expf(g.a_log[h]), g.a[tok], g.dt_bias[h]) : 0.0f;
+      const double G = wave_incl_scan_dpp((double)gt), Gend = readlane_d63(G);
+      const float eG = expf((float)G);
+      ((float *)(rec + kRecX))[lane] = eG * s_kn[lane];
+      ((float *)(rec + kRecQ))[lane] = eG * s_qn[lane];
+      ((float *)(rec + kRecR))[lane] = expf((float)(Gend - G)) * s_kn[lane];
+      if (lane == 0) *(float *)(rec + kRecEnd) = expf((float)Gend);
+      s_G[lane] = G;
+      s_beta[lane] = there ? sigmoid_ref(g.b[tok]) : 0.0f;
+      s_to[lane] = expf((float)(__shfl(G, lane | 15) - G));
+#pragma unroll
+      for (int j = 0; j < 3; j++) {
+        const double R = __shfl(G, 16 * j + 15);  // by all lanes
+        s_from[j * kChunk + lane] = (lane >> 4) > j ? expf((float)(G - R)) : 0.0f;
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    float x[kChunk];
+    // A^T and P, tile (i, j): rows s = 16 j + 4 kg + e, column t = 16 i + n16
 #pragma unroll
-    for (int t = 0; t < kChunk; t++) {
-      float acc[4] = {t == lane ? 1.0f : 0.0f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 4; i++)
 #pragma unroll
-      for (int s4 = 0; s4 < t; s4 += 4) {
-        const float4 r = *(const float4 *)(A + t * kChunk + s4);
-        acc[0] = __builtin_fmaf(-r.x, x[s4], acc[0]);
-        if (s4 + 1 < t) acc[1] = __builtin_fmaf(-r.y, x[s4 + 1], acc[1]);
-        if (s4 + 2 < t) acc[2] = __builtin_fmaf(-r.z, x[s4 + 2], acc[2]);
-        if (s4 + 3 < t) acc[3] = __builtin_fmaf(-r.w, x[s4 + 3], acc[3]);
+      for (int j = 0; j <= i; j++) {
+        const int u = i * (i + 1) / 2 + j, t = 16 * i + n16;
+        const v4f kk = s_pair[u * 64 + lane], qk = s_pair[(10 + u) * 64 + lane];
+        const float beta = s_beta[t];
+        float p[4];
+        float *at = s_a + u * 320;
+        if (j < i) {
+          const float f = s_from[j * kChunk + t];
+          const v4f e4 = *(const v4f *)(s_to + 16 * j + 4 * kg);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float x = f * e4[e];
+            at[(4 * kg + e) * 20 + n16] = beta * x * kk[e];
+            p[e] = x * qk[e];
+          }
+        } else {
+          const double G = s_G[t];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int r = 4 * kg + e;
+            const float x = r <= n16 ? expf((float)(G - s_G[16 * j + r])) : 0.0f;
+            at[r * 20 + n16] = r < n16 ? beta * x * kk[e] : 0.0f;
+            p[e] = r <= n16 ? x * qk[e] : 0.0f;
+          }
+        }
+        v2u p3[3];
+        split3(p, p3);
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+          *(v2u *)(rec + kRecP + 2 * (k * kTri + 128 * i * (i + 1) + n16 * 16 * (i + 1) + 16 * j + 4 * kg)) = p3[k];
       }
-      x[t] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-      rec[kRecInv + t * kChunk + lane] = x[t] * beta;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    // the diagonal tiles' inverses: lane (tile kg, column n16)
+    {
+      const float *at = s_a + (kg * (kg + 1) / 2 + kg) * 320;
+      float x[16];
+#pragma unroll
+      for (int r = 0; r < 16; r++) x[r] = r == n16 ? 1.0f : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 15; u++) {
+        float a16[16];
+#pragma unroll
+        for (int r = 4 * ((u + 1) / 4); r < 16; r += 4) *(v4f *)(a16 + r) = *(const v4f *)(at + u * 20 + r);
+#pragma unroll
+        for (int r = u + 1; r < 16; r++) x[r] = __builtin_fmaf(-a16[r], x[u], x[r]);
+      }
+      float *to = s_inv + kg * 320 + n16 * 20;
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) *(v4f *)(to + r) = v4f{x[r], x[r + 1], x[r + 2], x[r + 3]};
     }
-    // the next head's A goes where this one's is read
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    v4f inv[4];  // T_jj^T, row s = n16, as an A operand
+#pragma unroll
+    for (int j = 0; j < 4; j++) inv[j] = *(const v4f *)(s_inv + j * 320 + n16 * 20 + 4 * kg);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v4f T_[4];  // T_ij^T: row s = 4 kg + e, column t = n16
+#pragma unroll
+      for (int e = 0; e < 4; e++) T_[i][e] = s_inv[i * 320 + (4 * kg + e) * 20 + n16];
+#pragma unroll
+      for (int j = i - 1; j >= 0; j--) {
+        v4f sum = v4f{0.f, 0.f, 0.f, 0.f}, y = sum;
+#pragma unroll
+        for (int k = j + 1; k <= i; k++) {
+          const v4f ak = *(const v4f *)(s_a + (k * (k + 1) / 2 + j) * 320 + n16 * 20 + 4 * kg);
+#pragma unroll
+          for (int e = 0; e < 4; e++) sum = mfma_f32_16(ak[e], T_[k][e], sum);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) y = mfma_f32_16(-inv[j][e], sum[e], y);
+        T_[j] = y;
+      }
+#pragma unroll
+      for (int j = 0; j <= i; j++) {
+        const v4f beta = *(const v4f *)(s_beta + 16 * j + 4 * kg);
+        const float x[4] = {T_[j][0] * beta[0], T_[j][1] * beta[1], T_[j][2] * beta[2], T_[j][3] * beta[3]};
+        v2u p3[3];
+        split3(x, p3);
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+          *(v2u *)(rec + kRecInv + 2 * (k * kTri + 128 * i * (i + 1) + n16 * 16 * (i + 1) + 16 * j + 4 * kg)) = p3[k];
+      }
+    }
+    // the next head's values go where this one's are read
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
 }
-constexpr int kChunkLds = (2 * kChunk * kPitch + 2 * kChunk * kTri + 2 * kChunk) * 4;
-static_assert(4 * kChunk * kChunk <= 2 * kChunk * kPitch, "A of four waves lies over the rows");
 
 // ---------------------------------------------------------------------------
 // prompts: the state's walk over the chunks
 // ---------------------------------------------------------------------------
-// One workgroup of 4 waves a (value head, 32 value columns, sequence), chunk after
-// chunk.  The state slice lives in the accumulators of its update (32 key rows a
-// wave) and, for the products with q and k, in LDS.
-constexpr int kCol = kSlice + 4;  // pitch of [row][column] tiles
+// One workgroup of 8 waves a (value head, 32 value columns, sequence), chunk after
+// chunk in four steps with a barrier between them:
+//   keys, queries and the state's bf16 parts to LDS;
+//   x = v - e^G |k|^-1 (k S0) and e^G |q|^-1 (q S0), a 16 x 16 tile of each a wave;
+//   d = inverse x;
+//   o = that + P d, and S = e^G_63 S0 + k^T (e^(G_63 - G) |k|^-1 d), two tiles a wave.
+// The state slice stays in the accumulators of its update for the whole walk.  Every
+// B operand ([column][8 consecutive terms] in LDS) is written from results whose lanes
+// hold four consecutive rows of a column; k^T comes from k by the transposing LDS
+// load.  What a chunk reads from memory is loaded into registers while the chunk
+// before it is computed.
 template <class T>
-__global__ __launch_bounds__(256) void k_delta_scan(DeltaArgs g) {
-  extern __shared__ __align__(16) float lds[];
-  float *s_k = lds, *s_q = s_k + kChunk * kPitch, *s_s = s_q + kChunk * kPitch, *s_x = s_s + kKey * kCol,
-        *s_d = s_x + kChunk * kCol;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
-  const int nsl = g.dv / kSlice, h = blockIdx.x / nsl, col0 = (blockIdx.x % nsl) * kSlice, s = blockIdx.y;
+struct ScanLds {
+  static constexpr int NP = planes_of<T>();
+  static constexpr int kRows = kChunk * kPitchB;                // one plane of keys or queries
+  static constexpr int kPitchT = kChunk * 2 + 16;               // bytes of a column of 64 tokens
+  static constexpr int kTok = kSlice * kPitchT;                 // one plane of x or d
+  static constexpr int kState = kSlice * kPitchB;               // one plane of the state
+  static constexpr int kK = 0, kQ = NP * kRows, kS = 2 * NP * kRows;
+  static constexpr int kD = kS;                                 // d lies where the state was
+  static constexpr int kX = kS + 3 * kState, kR = kX + 3 * kTok, kAll = kR + 3 * kTok;
+};
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"
+typedef short v4s __attribute__((ext_vector_type(4)));
+// 16 lanes read four rows x 16 columns, four 16-bit values a lane, and get the four
+// rows of one column each
+__device__ __forceinline__ v2u lds_transposed(const void *p) {
+  return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                     (__attribute__((address_space(3))) v4s *)(const __attribute__((address_space(3))) void *)p));
+}
+#pragma clang diagnostic pop
+
+template <class T>
+__global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
+  typedef ScanLds<T> L;
+  constexpr int NP = L::NP, V = sizeof(T) / 2;
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n16 = lane & 15, kg = lane >> 4;
+  const int rt = wave & 3, ct = wave >> 2;  // row and column tile
+  const int nsl = g.dv / kSlice, units = g.vh * nsl, s = blockIdx.y;
+  // the slices of a value head, and the value heads of a key head, on one die: blocks
+  // go to the eight dies in turn
+  const int unit = units % 8 == 0 ? (blockIdx.x % 8) * (units / 8) + blockIdx.x / 8 : blockIdx.x;
+  const int h = unit / nsl, col = (unit % nsl) * kSlice + 16 * ct + n16;  // this lane's value column
   const int hk = h / (g.vh / g.kh);
-  const int rows = g.start[s + 1] - g.start[s];
+  const int rows = g.rows[s];
   const int c0 = g.chunk_first, c1 = min(c0 + g.chunks, (rows + kChunk - 1) / kChunk);
   if (c0 > 0 && c0 >= c1) return;  // an earlier pass ended this sequence
-  const size_t at = ((size_t)g.slot[s] * g.vh + h) * g.dk * g.dv + col0;
+  const size_t at = ((size_t)g.slot[s] * g.vh + h) * g.dk * g.dv + col;
   const float *from = c0 > 0 ? g.state_out : g.state;
-  v4f S[2][2];
+  v4f S[2];  // rows 32 rt + 16 i + 4 kg + e
 #pragma unroll
   for (int i = 0; i < 2; i++)
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+    for (int e = 0; e < 4; e++) {
+      const int r = 32 * rt + 16 * i + 4 * kg + e;
+      S[i][e] = r < g.dk ? from[at + (size_t)r * g.dv] : 0.0f;
+    }
+
+  // a chunk's part of this thread
+  const int lr = tid >> 3, lc = tid & 7;  // row, and pieces lc and lc + 8 of eight elements
+  v4u kraw[2][V], qraw[2][V], inv[2][3], pr[2][3];
+  T vv[4];
+  v4f fx, fq, fr;
+  float fe;
+  auto load = [&](int c) {
+    const int t0 = g.begin[s] + c * kChunk, n = min(kChunk, rows - c * kChunk);
+    const char *rec = g.rec + ((size_t)(g.chunk0[s] + c - c0) * g.vh + h) * kRec;
+    const T *kp = (const T *)g.k + (size_t)(t0 + lr) * g.k_stride + (size_t)hk * g.dk;
+    const T *qp = (const T *)g.q + (size_t)(t0 + lr) * g.q_stride + (size_t)hk * g.dk;
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int r = 32 * wave + 16 * i + 4 * kg + e;
-        S[i][j][e] = r < g.dk ? from[at + (size_t)r * g.dv + 16 * j + n16] : 0.0f;
+    for (int i = 0; i < 2; i++) {
+      const int d = 8 * (lc + 8 * i);
+      const bool in = lr < n && d < g.dk;
+#pragma unroll
+      for (int u = 0; u < V; u++) {
+        kraw[i][u] = in ? ((const v4u *)(kp + d))[u] : v4u{0, 0, 0, 0};
+        qraw[i][u] = in ? ((const v4u *)(qp + d))[u] : v4u{0, 0, 0, 0};
       }
-  for (int c = c0; c < c1; c++) {
-    const int t0 = g.start[s] + c * kChunk, n = min(kChunk, g.start[s + 1] - t0);
-    const float *rec = g.rec + ((size_t)(g.chunk0[s] + c - c0) * g.vh + h) * kRec;
-    stage_rows(s_k, (const T *)g.k + (size_t)t0 * g.k_stride + (size_t)hk * g.dk, g.k_stride, n, g.dk, nullptr);
-    stage_rows(s_q, (const T *)g.q + (size_t)t0 * g.q_stride + (size_t)hk * g.dk, g.q_stride, n, g.dk, nullptr);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int t = 16 * rt + 4 * kg + e;
+      vv[e] = t < n ? ((const T *)g.v)[(size_t)(t0 + t) * g.v_stride + (size_t)h * g.dv + col] : (T)0.0f;
+    }
+    // operands of the triangles' row tile: columns 32 i + 8 kg .., zero above the diagonal tile
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int j = 0; j < 2; j++)
+      for (int p = 0; p < 3; p++) {
+        const bool in = 32 * i + 8 * kg < 16 * (rt + 1);
+        const int off = 2 * (p * kTri + 128 * rt * (rt + 1) + n16 * 16 * (rt + 1) + 32 * i + 8 * kg);
+        inv[i][p] = in ? *(const v4u *)(rec + kRecInv + off) : v4u{0, 0, 0, 0};
+        pr[i][p] = in ? *(const v4u *)(rec + kRecP + off) : v4u{0, 0, 0, 0};
+      }
+    fx = *(const v4f *)(rec + kRecX + (16 * rt + 4 * kg) * 4);
+    fq = *(const v4f *)(rec + kRecQ + (16 * rt + 4 * kg) * 4);
+    fr = *(const v4f *)(rec + kRecR + (16 * rt + 4 * kg) * 4);
+    fe = *(const float *)(rec + kRecEnd);
+  };
+  // eight raw elements as NP bf16 pieces of 16 bytes
+  auto put_planes = [&](char *to, const v4u (&raw)[V]) {
+    if constexpr (NP == 1) {
+      *(v4u *)to = raw[0];
+    } else {
+      float x[8];
+      load8(x, (const T *)raw);
 #pragma unroll
-        for (int e = 0; e < 4; e++) s_s[(32 * wave + 16 * i + 4 * kg + e) * kCol + 16 * j + n16] = S[i][j][e];
+      for (int p = 0; p < NP; p++) {
+        v4u w;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+          const v2b b = v2b{(__bf16)x[2 * e], (__bf16)x[2 * e + 1]};
+          x[2 * e] -= (float)b[0];
+          x[2 * e + 1] -= (float)b[1];
+          w[e] = __builtin_bit_cast(unsigned, b);
+        }
+        *(v4u *)(to + p * L::kRows) = w;
+      }
+    }
+  };
+  // four consecutive rows of a column as three bf16 pieces of 8 bytes
+  auto put_split = [&](char *to, int plane, const v4f &x) {
+    const float x4[4] = {x[0], x[1], x[2], x[3]};
+    v2u p3[3];
+    split3(x4, p3);
+#pragma unroll
+    for (int p = 0; p < 3; p++) *(v2u *)(to + p * plane) = p3[p];
+  };
+
+  if (c0 < c1) load(c0);
+  for (int c = c0; c < c1; c++) {
+    const int t0 = g.begin[s] + c * kChunk, n = min(kChunk, rows - c * kChunk);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      put_planes(lds + L::kK + lr * kPitchB + 16 * (lc + 8 * i), kraw[i]);
+      put_planes(lds + L::kQ + lr * kPitchB + 16 * (lc + 8 * i), qraw[i]);
+      put_split(lds + L::kS + (16 * ct + n16) * kPitchB + 2 * (32 * rt + 16 * i + 4 * kg), L::kState, S[i]);
+    }
+    // the rest of this chunk's operands, before the registers take the next one's
+    v4u inv_[2][3], pr_[2][3];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int p = 0; p < 3; p++) inv_[i][p] = inv[i][p], pr_[i][p] = pr[i][p];
+    const v4f fx_ = fx, fq_ = fq, fr_ = fr;
+    const float fe_ = fe;
+    const v4f v_ = v4f{(float)vv[0], (float)vv[1], (float)vv[2], (float)vv[3]};
     __syncthreads();
-    // rows 16 wave .. of k S0 and q S0
-    v4f ks[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}}, o[2] = {ks[0], ks[0]};
-    for (int i = 0; i < g.dk; i += 16) {
-      const float4 kf = *(const float4 *)(s_k + (16 * wave + n16) * kPitch + i + 4 * kg);
-      const float4 qf = *(const float4 *)(s_q + (16 * wave + n16) * kPitch + i + 4 * kg);
+    if (c + 1 < c1) load(c + 1);
+    v4f ks = v4f{0.f, 0.f, 0.f, 0.f}, o = ks;
 #pragma unroll
-      for (int e = 0; e < 4; e++)
+    for (int d = 0; d < kKey; d += 32) {
+      if (d >= g.dk) break;
+      v4u kf[NP], qf[NP], sf[3];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const float sf = s_s[(i + 4 * kg + e) * kCol + 16 * j + n16];
-          ks[j] = mfma_f32_16(((const float *)&kf)[e], sf, ks[j]);
-          o[j] = mfma_f32_16(((const float *)&qf)[e], sf, o[j]);
+      for (int p = 0; p < NP; p++) {
+        kf[p] = *(const v4u *)(lds + L::kK + p * L::kRows + (16 * rt + n16) * kPitchB + 2 * d + 16 * kg);
+        qf[p] = *(const v4u *)(lds + L::kQ + p * L::kRows + (16 * rt + n16) * kPitchB + 2 * d + 16 * kg);
+      }
+#pragma unroll
+      for (int p = 0; p < 3; p++)
+        sf[p] = *(const v4u *)(lds + L::kS + p * L::kState + (16 * ct + n16) * kPitchB + 2 * d + 16 * kg);
+#pragma unroll
+      for (int p = 0; p < NP; p++)
+#pragma unroll
+        for (int r = 0; r + p < 3; r++) {
+          ks = mfma_b16(kf[p], sf[r], ks);
+          o = mfma_b16(qf[p], sf[r], o);
         }
     }
+    put_split(lds + L::kX + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, v_ - fx_ * ks);
+    o *= fq_;
+    __syncthreads();
+    auto triangle = [&](v4f acc, const v4u (&tri)[2][3], const char *b) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        if (2 * i > rt) break;
+        v4u bf[3];
+#pragma unroll
+        for (int p = 0; p < 3; p++) bf[p] = *(const v4u *)(b + p * L::kTok + (16 * ct + n16) * L::kPitchT + 64 * i + 16 * kg);
+#pragma unroll
+        for (int p = 0; p < 3; p++)
+#pragma unroll
+          for (int r = 0; r + p < 3; r++) acc = mfma_b16(tri[i][p], bf[r], acc);
+      }
+      return acc;
+    };
+    const v4f d = triangle(v4f{0.f, 0.f, 0.f, 0.f}, inv_, lds + L::kX);
+    put_split(lds + L::kD + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, d);
+    put_split(lds + L::kR + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, fr_ * d);
+    __syncthreads();
+    o = triangle(o, pr_, lds + L::kD);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const int t = 16 * wave + 4 * kg + e;
-      const float fx = rec[kRecX + t], fq = rec[kRecQ + t];
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const float v = t < n ? (float)((const T *)g.v)[(size_t)(t0 + t) * g.v_stride + (size_t)h * g.dv + col0 + 16 * j + n16] : 0.0f;
-        s_x[t * kCol + 16 * j + n16] = __builtin_fmaf(-fx, ks[j][e], v);
-        o[j][e] *= fq;
-      }
+      const int t = 16 * rt + 4 * kg + e;
+      if (t < n) ((T *)g.out)[((size_t)(t0 + t) * g.vh + h) * g.dv + col] = (T)o[e];
     }
-    __syncthreads();
-    // d = inverse x, lower triangular
-    v4f d[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
-    for (int i = 0; i <= wave; i++) {
-      const float4 f = *(const float4 *)(rec + kRecInv + (16 * wave + n16) * kChunk + 16 * i + 4 * kg);
+    S[0] *= fe_;
+    S[1] *= fe_;
 #pragma unroll
-      for (int e = 0; e < 4; e++)
+    for (int i = 0; i < 2; i++) {  // tokens 32 i ..
+      v4u bf[3];
 #pragma unroll
-        for (int j = 0; j < 2; j++)
-          d[j] = mfma_f32_16(((const float *)&f)[e], s_x[(16 * i + 4 * kg + e) * kCol + 16 * j + n16], d[j]);
-    }
+      for (int p = 0; p < 3; p++)
+        bf[p] = *(const v4u *)(lds + L::kR + p * L::kTok + (16 * ct + n16) * L::kPitchT + 64 * i + 16 * kg);
 #pragma unroll
-    for (int e = 0; e < 4; e++)
+      for (int m = 0; m < 2; m++)
 #pragma unroll
-      for (int j = 0; j < 2; j++) s_d[(16 * wave + 4 * kg + e) * kCol + 16 * j + n16] = d[j][e];
-    __syncthreads();
-    for (int i = 0; i <= wave; i++) {
-      const float4 f = *(const float4 *)(rec + kRecP + (16 * wave + n16) * kChunk + 16 * i + 4 * kg);
+        for (int p = 0; p < NP; p++) {
+          const char *kp = lds + L::kK + p * L::kRows + (32 * i + 8 * kg + (n16 >> 2)) * kPitchB +
+                           2 * (32 * rt + 16 * m + 4 * (n16 & 3));
+          const v2u lo = lds_transposed(kp), hi = lds_transposed(kp + 4 * kPitchB);
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-          o[j] = mfma_f32_16(((const float *)&f)[e], s_d[(16 * i + 4 * kg + e) * kCol + 16 * j + n16], o[j]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int t = 16 * wave + 4 * kg + e;
-      if (t < n)
-#pragma unroll
-        for (int j = 0; j < 2; j++) ((T *)g.out)[((size_t)(t0 + t) * g.vh + h) * g.dv + col0 + 16 * j + n16] = (T)o[j][e];
-    }
-    const float eg = rec[kRecEnd];
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < 2; j++) S[i][j] *= eg;
-    for (int i = 0; i < kChunk; i += 4) {
-      const int t = i + kg;
-      const float fr = rec[kRecR + t];
-      float df[2];
-#pragma unroll
-      for (int j = 0; j < 2; j++) df[j] = fr * s_d[t * kCol + 16 * j + n16];
-#pragma unroll
-      for (int m = 0; m < 2; m++) {
-        const float kf = s_k[t * kPitch + 32 * wave + 16 * m + n16];
-#pragma unroll
-        for (int j = 0; j < 2; j++) S[m][j] = mfma_f32_16(kf, df[j], S[m][j]);
-      }
+          for (int r = 0; r + p < 3; r++) S[m] = mfma_b16(v4u{lo[0], lo[1], hi[0], hi[1]}, bf[r], S[m]);
+        }
     }
     __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < 2; i++)
 #pragma unroll
-    for (int j = 0; j < 2; j++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int r = 32 * wave + 16 * i + 4 * kg + e;
-        if (r < g.dk) g.state_out[at + (size_t)r * g.dv + 16 * j + n16] = S[i][j][e];
-      }
+    for (int e = 0; e < 4; e++) {
+      const int r = 32 * rt + 16 * i + 4 * kg + e;
+      if (r < g.dk) g.state_out[at + (size_t)r * g.dv] = S[i][e];
+    }
 }
-constexpr int kScanLds = (2 * kChunk * kPitch + kKey * kCol + 2 * kChunk * kCol) * 4;
 
 // ---------------------------------------------------------------------------
 // host side
@@ -467,11 +699,13 @@ bool delta_ok(const char *name, const ColiDelta *d, const void *out, const void 
 
 template <class T>
 int launch_delta(const char *name, const DeltaArgs &g, int chunks, hipStream_t st) {
-  hipError_t e = hipFuncSetAttribute((const void *)k_delta_chunk<T>, hipFuncAttributeMaxDynamicSharedMemorySize, kChunkLds);
-  if (e == hipSuccess) e = hipFuncSetAttribute((const void *)k_delta_scan<T>, hipFuncAttributeMaxDynamicSharedMemorySize, kScanLds);
+  constexpr int chunk = chunk_lds<T>(), scan = ScanLds<T>::kAll;
+  static_assert(chunk <= 160 * 1024 && scan <= 160 * 1024, "LDS of a compute unit");
+  hipError_t e = hipFuncSetAttribute((const void *)k_delta_chunk<T>, hipFuncAttributeMaxDynamicSharedMemorySize, chunk);
+  if (e == hipSuccess) e = hipFuncSetAttribute((const void *)k_delta_scan<T>, hipFuncAttributeMaxDynamicSharedMemorySize, scan);
   if (e != hipSuccess) return fail_hip(name, e);
-  if (chunks) k_delta_chunk<T><<<dim3(chunks, g.kh), 256, kChunkLds, st>>>(g);
-  k_delta_scan<T><<<dim3(g.vh * (g.dv / kSlice), g.seqs), 256, kScanLds, st>>>(g);
+  if (chunks) k_delta_chunk<T><<<dim3(chunks, g.kh), 256, chunk, st>>>(g);
+  k_delta_scan<T><<<dim3(g.vh * (g.dv / kSlice), g.seqs), 512, scan, st>>>(g);
   return 0;
 }
 
@@ -534,29 +768,36 @@ extern "C" int coli_cuda_delta_prompt(ColiCuda *ctx, const ColiDelta *d, void *o
   g.q_stride = d->q_stride, g.k_stride = d->k_stride, g.v_stride = d->v_stride;
   g.kh = d->key_heads, g.vh = d->value_heads, g.dk = d->key_dim, g.dv = d->value_dim;
   // records of a pass: 512 MiB, a chunk of every sequence at least
-  const size_t chunk_bytes = (size_t)g.vh * kRec * sizeof(float);
+  const size_t chunk_bytes = (size_t)g.vh * kRec;
   for (int s0 = 0; s0 < sequences; s0 += kSeqs) {
     const int n = sequences - s0 < kSeqs ? sequences - s0 : kSeqs;
     long long per = (long long)((512u << 20) / chunk_bytes) / n;
     if (per < 1) per = 1;
-    int longest = 0;
+    // long sequences first: their walk takes longest
     for (int s = 0; s < n; s++) {
-      const int c = (int)(((long long)start[s0 + s + 1] - start[s0 + s] + kChunk - 1) / kChunk);
-      if (c > longest) longest = c;
+      const int rows = start[s0 + s + 1] - start[s0 + s];
+      int i = s;
+      for (; i > 0 && g.rows[i - 1] < rows; i--) {
+        g.begin[i] = g.begin[i - 1];
+        g.rows[i] = g.rows[i - 1];
+        g.slot[i] = g.slot[i - 1];
+      }
+      g.begin[i] = start[s0 + s];
+      g.rows[i] = rows;
+      g.slot[i] = slot[s0 + s];
     }
+    const int longest = (int)(((long long)g.rows[0] + kChunk - 1) / kChunk);
     g.chunks = per < longest ? (int)per : longest;
-    memcpy(g.start, start + s0, (n + 1) * sizeof(int));
-    memcpy(g.slot, slot + s0, n * sizeof(int));
     g.seqs = n;
     for (g.chunk_first = 0; g.chunk_first == 0 || g.chunk_first < longest; g.chunk_first += g.chunks) {
       for (int s = 0; s < n; s++) {
-        int c = (int)(((long long)g.start[s + 1] - g.start[s] + kChunk - 1) / kChunk) - g.chunk_first;
+        int c = (int)(((long long)g.rows[s] + kChunk - 1) / kChunk) - g.chunk_first;
         if (c > g.chunks) c = g.chunks;
         g.chunk0[s + 1] = g.chunk0[s] + (c > 0 ? c : 0);
       }
       const int chunks = g.chunk0[n];
       if (ensure_scratch(ctx, kScrDelta, (size_t)(chunks ? chunks : 1) * chunk_bytes, name)) return -1;
-      g.rec = (float *)ctx->scratch[kScrDelta];
+      g.rec = (char *)ctx->scratch[kScrDelta];
       const int rc = d->type == COLI_TYPE_F32   ? launch_delta<float>(name, g, chunks, ctx->stream)
                      : d->type == COLI_TYPE_F16 ? launch_delta<_Float16>(name, g, chunks, ctx->stream)
                                                 : launch_delta<__bf16>(name, g, chunks, ctx->stream);
