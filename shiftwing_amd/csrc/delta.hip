@@ -36,14 +36,24 @@ constexpr int kSlice = 32;  // value columns of a k_delta_scan workgroup
 // cores, without the terms below 2^-24, are fp32 products in all but rounding, at 3
 // (one factor bf16) to 6 instructions of 16 cycles where the fp32 matrix cores take 8
 // of 32 for the same tile.
-constexpr int kTri = 10 * 256;  // elements of a 64 x 64 lower triangle in 16 x 16 tiles
-// One (chunk, value head) record of k_delta_chunk: the inverse of 1 + A times beta, and
-// P, as three bf16 triangles each; then per token e^G |k|^-1, e^G |q|^-1 key_dim^-1/2
-// and e^(G_63 - G) |k|^-1, then e^G_63, in fp32.  A triangle's row tile i is
-// [16 rows][16 (i + 1)] at 128 i (i + 1), which gives a lane its matrix operand in one load.
-constexpr int kRecInv = 0, kRecP = 3 * kTri * 2, kRecX = 2 * kRecP, kRecQ = kRecX + kChunk * 4,
-              kRecR = kRecQ + kChunk * 4, kRecEnd = kRecR + kChunk * 4, kRec = kRecEnd + 16;  // bytes
-static_assert(kRec % 16 == 0, "records are 16-byte aligned");
+constexpr int kTri = 12 * 256;  // elements of a 64 x 64 lower triangle in 16 x 16 tiles, two of them zero
+// Outputs of 16-bit types take two parts a factor, terms down to 2^-16 relative: far
+// below their rounding, 2^-8 or 2^-11; states always all three.
+// One (chunk, value head) record of k_delta_chunk: the inverse of 1 + A times beta as
+// three bf16 triangles, P as one for each part that outputs take; then per token e^G |k|^-1, e^G |q|^-1 key_dim^-1/2
+// and e^(G_63 - G) |k|^-1, then e^G_63, in fp32.  A triangle's row tiles are
+// [16 rows][32 columns], twice, then [16][64], twice (zero above the diagonal): a lane
+// has its matrix operand of 32 columns in one load.
+template <class T>
+struct Rec {
+  static constexpr int kParts = sizeof(T) == 4 ? 3 : 2;  // of a factor of the outputs
+  static constexpr int kInv = 0, kP = 3 * kTri * 2, kX = kP + kParts * kTri * 2, kQ = kX + kChunk * 4, kR = kQ + kChunk * 4,
+                       kEnd = kR + kChunk * 4, kBytes = kEnd + 16;
+  static_assert(kBytes % 16 == 0, "records are 16-byte aligned");
+};
+__device__ __forceinline__ constexpr int tri_at(int i, int row) {  // element of row tile i's row, column 0
+  return i < 2 ? 512 * i + 32 * row : 1024 * (i - 1) + 64 * row;
+}
 
 struct DeltaArgs {
   const void *q, *k, *v;
@@ -222,7 +232,7 @@ struct ChunkLds {
   static constexpr int kNorms = kPairs + 20 * 1024;      // |k|^-1, |q|^-1 key_dim^-1/2
   static constexpr int kWork = kNorms + 2 * kChunk * 4;  // raw rows, then per wave:
   static constexpr int kTile = 16 * 20 * 4;              // a 16 x 16 fp32 tile, rows of 80 bytes
-  static constexpr int kWave = 14 * kTile + kChunk * (8 + 4 * 5);  // 10 tiles of A, 4 of the inverse, G, beta, factors
+  static constexpr int kWave = 10 * kTile + kChunk * (8 + 4 * 5);  // tiles of A, G, beta, factors
 };
 template <class T>
 constexpr int chunk_lds() {
@@ -233,6 +243,7 @@ constexpr int chunk_lds() {
 template <class T>
 __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
   typedef ChunkLds L;
+  typedef Rec<T> R;
   constexpr int kPitch = sizeof(T) == 4 ? kPitchF : kPitchB;
   extern __shared__ __align__(16) char lds[];
   v4f *s_pair = (v4f *)(lds + L::kPairs);
@@ -243,6 +254,11 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
   const int first = (blockIdx.x - g.chunk0[s] + g.chunk_first) * kChunk;
   const int t0 = g.begin[s] + first, n = min(kChunk, g.rows[s] - first);
 
+  // a wave's first head's gates, on their way while the rows are
+  const int rep = g.vh / g.kh;
+  const size_t gate_at = (size_t)(t0 + min(lane, n - 1)) * g.vh;
+  const int h_first = hk * rep + (wave < rep ? wave : 0);
+  float a_ = g.a[gate_at + h_first], b_ = g.b[gate_at + h_first], al_ = g.a_log[h_first], dt_ = g.dt_bias[h_first];
   // raw rows, zero beyond the sequence's end and beyond key_dim
   {
     const int t = threadIdx.x >> 2, p = threadIdx.x & 3;
@@ -294,26 +310,25 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
   }
   __syncthreads();
 
-  const int rep = g.vh / g.kh;
   char *mine = lds + L::kWork + wave * L::kWave;
-  float *s_a = (float *)mine, *s_inv = s_a + 10 * 320;  // tiles [row s][t] of A^T, of the diagonal inverses' transposes
-  double *s_G = (double *)(s_inv + 4 * 320);
+  float *s_a = (float *)mine;  // tiles [row s][t] of A^T; the diagonal ones become their inverses' transposes
+  double *s_G = (double *)(s_a + 10 * 320);
   float *s_beta = (float *)(s_G + kChunk), *s_to = s_beta + kChunk, *s_from = s_to + kChunk;  // s_from [3][64]
   for (int w = wave; w < rep; w += 4) {
     const int h = hk * rep + w;
-    char *rec = g.rec + ((size_t)blockIdx.x * g.vh + h) * kRec;
+    char *rec = g.rec + ((size_t)blockIdx.x * g.vh + h) * R::kBytes;
     {
       const bool there = lane < n;
-      const size_t tok = (size_t)(t0 + (there ? lane : 0)) * g.vh + h;
-      const float gt = there ? log_decay(expf(g.a_log[h]), g.a[tok], g.dt_bias[h]) : 0.0f;
+      if (w != wave) a_ = g.a[gate_at + h], b_ = g.b[gate_at + h], al_ = g.a_log[h], dt_ = g.dt_bias[h];
+      const float gt = there ? log_decay(expf(al_), a_, dt_) : 0.0f;
       const double G = wave_incl_scan_dpp((double)gt), Gend = readlane_d63(G);
       const float eG = expf((float)G);
-      ((float *)(rec + kRecX))[lane] = eG * s_kn[lane];
-      ((float *)(rec + kRecQ))[lane] = eG * s_qn[lane];
-      ((float *)(rec + kRecR))[lane] = expf((float)(Gend - G)) * s_kn[lane];
-      if (lane == 0) *(float *)(rec + kRecEnd) = expf((float)Gend);
+      ((float *)(rec + R::kX))[lane] = eG * s_kn[lane];
+      ((float *)(rec + R::kQ))[lane] = eG * s_qn[lane];
+      ((float *)(rec + R::kR))[lane] = expf((float)(Gend - G)) * s_kn[lane];
+      if (lane == 0) *(float *)(rec + R::kEnd) = expf((float)Gend);
       s_G[lane] = G;
-      s_beta[lane] = there ? sigmoid_ref(g.b[tok]) : 0.0f;
+      s_beta[lane] = there ? sigmoid_ref(b_) : 0.0f;
       s_to[lane] = expf((float)(__shfl(G, lane | 15) - G));
 #pragma unroll
       for (int j = 0; j < 3; j++) {
@@ -323,6 +338,13 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; i += 2)  // the tiles right of the diagonal that a 32-column operand holds
+#pragma unroll
+      for (int k = 0; k < 3; k++) {
+        if (k < R::kParts) *(v2u *)(rec + R::kP + 2 * (k * kTri + tri_at(i, n16) + 16 * (i + 1) + 4 * kg)) = v2u{0, 0};
+        *(v2u *)(rec + R::kInv + 2 * (k * kTri + tri_at(i, n16) + 16 * (i + 1) + 4 * kg)) = v2u{0, 0};
+      }
     // A^T and P, tile (i, j): rows s = 16 j + 4 kg + e, column t = 16 i + n16
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -355,14 +377,14 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
         v2u p3[3];
         split3(p, p3);
 #pragma unroll
-        for (int k = 0; k < 3; k++)
-          *(v2u *)(rec + kRecP + 2 * (k * kTri + 128 * i * (i + 1) + n16 * 16 * (i + 1) + 16 * j + 4 * kg)) = p3[k];
+        for (int k = 0; k < R::kParts; k++)
+          *(v2u *)(rec + R::kP + 2 * (k * kTri + tri_at(i, n16) + 16 * j + 4 * kg)) = p3[k];
       }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     // the diagonal tiles' inverses: lane (tile kg, column n16)
     {
-      const float *at = s_a + (kg * (kg + 1) / 2 + kg) * 320;
+      float *at = s_a + (kg * (kg + 1) / 2 + kg) * 320;
       float x[16];
 #pragma unroll
       for (int r = 0; r < 16; r++) x[r] = r == n16 ? 1.0f : 0.0f;
@@ -374,7 +396,9 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
 #pragma unroll
         for (int r = u + 1; r < 16; r++) x[r] = __builtin_fmaf(-a16[r], x[u], x[r]);
       }
-      float *to = s_inv + kg * 320 + n16 * 20;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      float *to = at + n16 * 20;
 #pragma unroll
       for (int r = 0; r < 16; r += 4) *(v4f *)(to + r) = v4f{x[r], x[r + 1], x[r + 2], x[r + 3]};
     }
@@ -382,12 +406,12 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
     __builtin_amdgcn_wave_barrier();
     v4f inv[4];  // T_jj^T, row s = n16, as an A operand
 #pragma unroll
-    for (int j = 0; j < 4; j++) inv[j] = *(const v4f *)(s_inv + j * 320 + n16 * 20 + 4 * kg);
+    for (int j = 0; j < 4; j++) inv[j] = *(const v4f *)(s_a + (j * (j + 1) / 2 + j) * 320 + n16 * 20 + 4 * kg);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       v4f T_[4];  // T_ij^T: row s = 4 kg + e, column t = n16
 #pragma unroll
-      for (int e = 0; e < 4; e++) T_[i][e] = s_inv[i * 320 + (4 * kg + e) * 20 + n16];
+      for (int e = 0; e < 4; e++) T_[i][e] = s_a[(i * (i + 1) / 2 + i) * 320 + (4 * kg + e) * 20 + n16];
 #pragma unroll
       for (int j = i - 1; j >= 0; j--) {
         v4f sum = v4f{0.f, 0.f, 0.f, 0.f}, y = sum;
@@ -409,7 +433,7 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
         split3(x, p3);
 #pragma unroll
         for (int k = 0; k < 3; k++)
-          *(v2u *)(rec + kRecInv + 2 * (k * kTri + 128 * i * (i + 1) + n16 * 16 * (i + 1) + 16 * j + 4 * kg)) = p3[k];
+          *(v2u *)(rec + R::kInv + 2 * (k * kTri + tri_at(i, n16) + 16 * j + 4 * kg)) = p3[k];
       }
     }
     // the next head's values go where this one's are read
@@ -443,6 +467,9 @@ struct ScanLds {
   static constexpr int kD = kS;                                 // d lies where the state was
   static constexpr int kX = kS + 3 * kState, kR = kX + 3 * kTok, kAll = kR + 3 * kTok;
 };
+// A barrier that waits for this wave's LDS accesses alone: __syncthreads would also
+// wait for the next chunk's loads in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Wint-to-pointer-cast"
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -457,10 +484,11 @@ __device__ __forceinline__ v2u lds_transposed(const void *p) {
 template <class T>
 __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
   typedef ScanLds<T> L;
+  typedef Rec<T> R;
   constexpr int NP = L::NP, V = sizeof(T) / 2;
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n16 = lane & 15, kg = lane >> 4;
-  const int rt = wave & 3, ct = wave >> 2;  // row and column tile
+  const int rt = __builtin_amdgcn_readfirstlane(wave & 3), ct = __builtin_amdgcn_readfirstlane(wave >> 2);  // row and column tile
   const int nsl = g.dv / kSlice, units = g.vh * nsl, s = blockIdx.y;
   // the slices of a value head, and the value heads of a key head, on one die: blocks
   // go to the eight dies in turn
@@ -481,46 +509,63 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
       S[i][e] = r < g.dk ? from[at + (size_t)r * g.dv] : 0.0f;
     }
 
-  // a chunk's part of this thread
+  // a chunk's part of this thread, and where the next one's lies
   const int lr = tid >> 3, lc = tid & 7;  // row, and pieces lc and lc + 8 of eight elements
-  v4u kraw[2][V], qraw[2][V], inv[2][3], pr[2][3];
+  const size_t row0 = (size_t)g.begin[s] + (size_t)c0 * kChunk;
+  const T *kp = (const T *)g.k + (row0 + lr) * g.k_stride + (size_t)hk * g.dk + 8 * lc;
+  const T *qp = (const T *)g.q + (row0 + lr) * g.q_stride + (size_t)hk * g.dk + 8 * lc;
+  const T *vp = (const T *)g.v + (row0 + 16 * rt + 4 * kg) * g.v_stride + (size_t)h * g.dv + col;
+  T *op = (T *)g.out + ((row0 + 16 * rt + 4 * kg) * g.vh + h) * g.dv + col;
+  const size_t orow = (size_t)g.vh * g.dv;
+  const char *rec = g.rec + ((size_t)g.chunk0[s] * g.vh + h) * R::kBytes;
+  const int tri = 2 * (tri_at(rt, n16) + 8 * kg), tok = 4 * (16 * rt + 4 * kg);
+  v4u kraw[2][V], qraw[2][V], inv[2][3], pr[2][R::kParts];
   T vv[4];
   v4f fx, fq, fr;
   float fe;
-  auto load = [&](int c) {
-    const int t0 = g.begin[s] + c * kChunk, n = min(kChunk, rows - c * kChunk);
-    const char *rec = g.rec + ((size_t)(g.chunk0[s] + c - c0) * g.vh + h) * kRec;
-    const T *kp = (const T *)g.k + (size_t)(t0 + lr) * g.k_stride + (size_t)hk * g.dk;
-    const T *qp = (const T *)g.q + (size_t)(t0 + lr) * g.q_stride + (size_t)hk * g.dk;
+  auto load_rows = [&](int c) {
+    const int n = rows - c * kChunk;
+    if (n >= kChunk && g.dk == kKey) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int u = 0; u < V; u++) {
+          kraw[i][u] = ((const v4u *)(kp + 64 * i))[u];
+          qraw[i][u] = ((const v4u *)(qp + 64 * i))[u];
+        }
+#pragma unroll
+      for (int e = 0; e < 4; e++) vv[e] = vp[(size_t)e * g.v_stride];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const bool in = lr < n && 8 * lc + 64 * i < g.dk;
+#pragma unroll
+        for (int u = 0; u < V; u++) {
+          kraw[i][u] = in ? ((const v4u *)(kp + 64 * i))[u] : v4u{0, 0, 0, 0};
+          qraw[i][u] = in ? ((const v4u *)(qp + 64 * i))[u] : v4u{0, 0, 0, 0};
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) vv[e] = 16 * rt + 4 * kg + e < n ? vp[(size_t)e * g.v_stride] : (T)0.0f;
+    }
+    kp += (size_t)kChunk * g.k_stride;
+    qp += (size_t)kChunk * g.q_stride;
+    vp += (size_t)kChunk * g.v_stride;
+  };
+  auto load_triangle = [&](auto &to, int which) {
+    constexpr int parts = sizeof(to[0]) / sizeof(v4u);
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const int d = 8 * (lc + 8 * i);
-      const bool in = lr < n && d < g.dk;
+      if (2 * i > rt) break;
 #pragma unroll
-      for (int u = 0; u < V; u++) {
-        kraw[i][u] = in ? ((const v4u *)(kp + d))[u] : v4u{0, 0, 0, 0};
-        qraw[i][u] = in ? ((const v4u *)(qp + d))[u] : v4u{0, 0, 0, 0};
-      }
+      for (int p = 0; p < parts; p++) to[i][p] = *(const v4u *)(rec + which + 2 * p * kTri + tri + 64 * i);
     }
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int t = 16 * rt + 4 * kg + e;
-      vv[e] = t < n ? ((const T *)g.v)[(size_t)(t0 + t) * g.v_stride + (size_t)h * g.dv + col] : (T)0.0f;
-    }
-    // operands of the triangles' row tile: columns 32 i + 8 kg .., zero above the diagonal tile
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int p = 0; p < 3; p++) {
-        const bool in = 32 * i + 8 * kg < 16 * (rt + 1);
-        const int off = 2 * (p * kTri + 128 * rt * (rt + 1) + n16 * 16 * (rt + 1) + 32 * i + 8 * kg);
-        inv[i][p] = in ? *(const v4u *)(rec + kRecInv + off) : v4u{0, 0, 0, 0};
-        pr[i][p] = in ? *(const v4u *)(rec + kRecP + off) : v4u{0, 0, 0, 0};
-      }
-    fx = *(const v4f *)(rec + kRecX + (16 * rt + 4 * kg) * 4);
-    fq = *(const v4f *)(rec + kRecQ + (16 * rt + 4 * kg) * 4);
-    fr = *(const v4f *)(rec + kRecR + (16 * rt + 4 * kg) * 4);
-    fe = *(const float *)(rec + kRecEnd);
+  };
+  auto load_factors = [&] {
+    fx = *(const v4f *)(rec + R::kX + tok);
+    fq = *(const v4f *)(rec + R::kQ + tok);
+    fr = *(const v4f *)(rec + R::kR + tok);
+    fe = *(const float *)(rec + R::kEnd);
   };
   // eight raw elements as NP bf16 pieces of 16 bytes
   auto put_planes = [&](char *to, const v4u (&raw)[V]) {
@@ -545,34 +590,34 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
     }
   };
   // four consecutive rows of a column as three bf16 pieces of 8 bytes
-  auto put_split = [&](char *to, int plane, const v4f &x) {
+  auto put_split = [&](char *to, int plane, const v4f &x, int parts = 3) {
     const float x4[4] = {x[0], x[1], x[2], x[3]};
     v2u p3[3];
     split3(x4, p3);
 #pragma unroll
-    for (int p = 0; p < 3; p++) *(v2u *)(to + p * plane) = p3[p];
+    for (int p = 0; p < 3; p++)
+      if (p < parts) *(v2u *)(to + p * plane) = p3[p];
   };
 
-  if (c0 < c1) load(c0);
+  if (c0 < c1) {
+    load_rows(c0);
+    load_triangle(inv, R::kInv);
+    load_triangle(pr, R::kP);
+    load_factors();
+  }
   for (int c = c0; c < c1; c++) {
-    const int t0 = g.begin[s] + c * kChunk, n = min(kChunk, rows - c * kChunk);
+    const int n = rows - c * kChunk;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       put_planes(lds + L::kK + lr * kPitchB + 16 * (lc + 8 * i), kraw[i]);
       put_planes(lds + L::kQ + lr * kPitchB + 16 * (lc + 8 * i), qraw[i]);
       put_split(lds + L::kS + (16 * ct + n16) * kPitchB + 2 * (32 * rt + 16 * i + 4 * kg), L::kState, S[i]);
     }
-    // the rest of this chunk's operands, before the registers take the next one's
-    v4u inv_[2][3], pr_[2][3];
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int p = 0; p < 3; p++) inv_[i][p] = inv[i][p], pr_[i][p] = pr[i][p];
-    const v4f fx_ = fx, fq_ = fq, fr_ = fr;
-    const float fe_ = fe;
     const v4f v_ = v4f{(float)vv[0], (float)vv[1], (float)vv[2], (float)vv[3]};
-    __syncthreads();
-    if (c + 1 < c1) load(c + 1);
+    lds_barrier();
+    // the next chunk's loads go out a few a step: a wave waits to issue when many are
+    if (c + 1 < c1) load_rows(c + 1);
+    rec += (size_t)g.vh * R::kBytes;
     v4f ks = v4f{0.f, 0.f, 0.f, 0.f}, o = ks;
 #pragma unroll
     for (int d = 0; d < kKey; d += 32) {
@@ -591,36 +636,47 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
 #pragma unroll
         for (int r = 0; r + p < 3; r++) {
           ks = mfma_b16(kf[p], sf[r], ks);
-          o = mfma_b16(qf[p], sf[r], o);
+          if (r + p < R::kParts) o = mfma_b16(qf[p], sf[r], o);
         }
     }
-    put_split(lds + L::kX + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, v_ - fx_ * ks);
-    o *= fq_;
-    __syncthreads();
-    auto triangle = [&](v4f acc, const v4u (&tri)[2][3], const char *b) {
+    put_split(lds + L::kX + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, v_ - fx * ks);
+    o *= fq;
+    lds_barrier();
+    auto triangle = [&](v4f acc, const auto &tr, const char *b) {
+      constexpr int parts = sizeof(tr[0]) / sizeof(v4u);
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         if (2 * i > rt) break;
-        v4u bf[3];
+        v4u bf[parts];
 #pragma unroll
-        for (int p = 0; p < 3; p++) bf[p] = *(const v4u *)(b + p * L::kTok + (16 * ct + n16) * L::kPitchT + 64 * i + 16 * kg);
+        for (int p = 0; p < parts; p++) bf[p] = *(const v4u *)(b + p * L::kTok + (16 * ct + n16) * L::kPitchT + 64 * i + 16 * kg);
 #pragma unroll
-        for (int p = 0; p < 3; p++)
+        for (int p = 0; p < parts; p++)
 #pragma unroll
-          for (int r = 0; r + p < 3; r++) acc = mfma_b16(tri[i][p], bf[r], acc);
+          for (int r = 0; r + p < parts; r++) acc = mfma_b16(tr[i][p], bf[r], acc);
       }
       return acc;
     };
-    const v4f d = triangle(v4f{0.f, 0.f, 0.f, 0.f}, inv_, lds + L::kX);
-    put_split(lds + L::kD + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, d);
-    put_split(lds + L::kR + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, fr_ * d);
-    __syncthreads();
-    o = triangle(o, pr_, lds + L::kD);
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int t = 16 * rt + 4 * kg + e;
-      if (t < n) ((T *)g.out)[((size_t)(t0 + t) * g.vh + h) * g.dv + col] = (T)o[e];
+    const v4f d = triangle(v4f{0.f, 0.f, 0.f, 0.f}, inv, lds + L::kX);
+    if (c + 1 < c1) load_triangle(inv, R::kInv);
+    put_split(lds + L::kD + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, d, R::kParts);
+    put_split(lds + L::kR + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, fr * d);
+    lds_barrier();
+    o = triangle(o, pr, lds + L::kD);
+    const float fe_ = fe;
+    if (c + 1 < c1) {
+      load_triangle(pr, R::kP);
+      load_factors();
     }
+    if (n >= kChunk) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) op[e * orow] = (T)o[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (16 * rt + 4 * kg + e < n) op[e * orow] = (T)o[e];
+    }
+    op += kChunk * orow;
     S[0] *= fe_;
     S[1] *= fe_;
 #pragma unroll
@@ -640,7 +696,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
           for (int r = 0; r + p < 3; r++) S[m] = mfma_b16(v4u{lo[0], lo[1], hi[0], hi[1]}, bf[r], S[m]);
         }
     }
-    __syncthreads();
+    lds_barrier();
   }
 #pragma unroll
   for (int i = 0; i < 2; i++)
@@ -768,7 +824,7 @@ extern "C" int coli_cuda_delta_prompt(ColiCuda *ctx, const ColiDelta *d, void *o
   g.q_stride = d->q_stride, g.k_stride = d->k_stride, g.v_stride = d->v_stride;
   g.kh = d->key_heads, g.vh = d->value_heads, g.dk = d->key_dim, g.dv = d->value_dim;
   // records of a pass: 512 MiB, a chunk of every sequence at least
-  const size_t chunk_bytes = (size_t)g.vh * kRec;
+  const size_t chunk_bytes = (size_t)g.vh * (d->type == COLI_TYPE_F32 ? Rec<float>::kBytes : Rec<__bf16>::kBytes);
   for (int s0 = 0; s0 < sequences; s0 += kSeqs) {
     const int n = sequences - s0 < kSeqs ? sequences - s0 : kSeqs;
     long long per = (long long)((512u << 20) / chunk_bytes) / n;
