@@ -30,6 +30,11 @@ struct PageMap {
   long long stride;
   int row;  // elements of one position: kv_heads * head_dim
 };
+// A wave's page id by a scalar load (the table does not change during a kernel): a
+// vector load would be waited for at once, to make its value scalar.
+__device__ __forceinline__ int scalar_id(const int *tab, int pg) {
+  return ((const __attribute__((address_space(4))) int *)tab)[pg];
+}
 // Element offset of position p of the sequence whose table row is `tab`; -1 where
 // the table names no page.
 __device__ __forceinline__ long long cell(const PageMap &m, const int *tab, int p) {
@@ -456,13 +461,14 @@ struct PromptArgs {
   float *po, *pm, *pl;  // partial records [split][row - row0][head] (null: one split)
   long long gate_stride;
   int gate_head, nh, nkv, G, seqs, first_seq, splits, rows;
-  float scale;  // scale * log2(e)
+  float scale;      // |scale| * log2(e)
+  unsigned q_sign;  // sign bits of a register of queries where scale is negative
   FastDiv by_group;
   PageMap map;
   int start[kSeqs + 1], len[kSeqs], tile0[kSeqs + 1];  // sequence s's tiles are tile0[s] .. tile0[s + 1] - 1
 };
 
-__device__ float g_zero_row[256];  // never written: what copies of absent positions read
+__device__ float g_zero_row[256];  // never written: what copies of absent positions read (a row of 1 KB at most)
 
 __device__ __forceinline__ v16f mfma_f32_32(float a, float b, v16f c) {
   return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
@@ -484,13 +490,16 @@ __device__ __forceinline__ v2u lds_transposed(unsigned at) {
 template <class T, int HD>
 struct PromptShape {
   static constexpr bool B16 = sizeof(T) == 2;
-  static constexpr int kWaves = 4;
+  // rows of a wave, the columns of its matrix instructions: 32 (32x32x16), or 16
+  // (16x16x32) where the outputs of 32 would leave a SIMD one wave
+  static constexpr int kCols = B16 && HD == 256 ? 16 : 32;
+  static constexpr int kWaves = 128 / kCols;
   static constexpr int kKeys = B16 ? 64 : 32;               // positions of a tile
   static constexpr int kRowBytes = HD * (int)sizeof(T);
   static constexpr int kTileBytes = kKeys * kRowBytes;      // of one matrix
   static constexpr int kLds = 4 * kTileBytes + 16;          // K and V, two buffers, flags
-  static constexpr int kRows = 32 * kWaves;                 // (token, head) rows of a workgroup
-  static constexpr int kPerCu = kLds <= 80 * 1024 ? 2 : 1;  // workgroups that a compute unit holds
+  static constexpr int kRows = 128;                         // (token, head) rows of a workgroup
+  static constexpr int kPerSimd = B16 || HD < 256 ? 2 : 1;  // waves of a SIMD
 };
 
 // One workgroup a (tile of rows, kv head, split of the tile's positions).  A row is
@@ -506,20 +515,23 @@ struct PromptShape {
 // (16 bits) or as single values (fp32).
 // LDS rows are stored with their 16-byte chunks exchanged by an XOR with the row
 // number, which spreads every access over all banks.
-template <class T, int HD>
-__global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, HD>::kPerCu)) void k_paged_prompt(PromptArgs a) {
+// RUN: pages hold whole runs of the WR positions that a wave copies, whose page is
+// then looked up once, by a scalar load.
+template <class T, int HD, bool RUN>
+__global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, HD>::kPerSimd)) void k_paged_prompt(PromptArgs a) {
   typedef PromptShape<T, HD> Sh;
   constexpr bool B16 = Sh::B16;
   constexpr int KT = Sh::kKeys, RB = Sh::kRowBytes, CPR = RB / 16, NI = Sh::kTileBytes / 1024 / Sh::kWaves;
-  constexpr int NS = KT / 32;      // 32-position subtiles
-  constexpr int ND = HD / 32;      // 32-dim tiles
-  constexpr int KC = HD * (int)sizeof(T) / 32;  // 16-byte chunks of half a row: Q registers x 4
+  constexpr int C = Sh::kCols, NG = 64 / C, NA = C * C / 64;  // lane groups, registers of a C x C result
+  constexpr int NS = KT / C, ND = HD / C;                     // tiles of positions, of dims
+  constexpr int KC = CPR / NG;                                // 16-byte chunks of a lane's part of a row
+  typedef float Acc __attribute__((ext_vector_type(NA)));     // register i: row 4 NG (i / 4) + 4 g + i % 4
   extern __shared__ __align__(1024) unsigned char smem[];
-  // tag of the latest tile of its residue with an absent page: written two tiles
-  // ahead, so four residues keep the tag that others may still read
+  // tag of the latest tile of its residue with an absent page: written a tile ahead,
+  // while others may still read the one before
   int *s_bad = (int *)(smem + 4 * Sh::kTileBytes);
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31,
-            hf = lane >> 5;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & (C - 1),
+            g = lane / C;
   const int kvh = blockIdx.y, split = blockIdx.z;
   // late tiles see most and go first
   const int tile = gridDim.x - 1 - blockIdx.x;
@@ -537,13 +549,13 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, 
   const int key_first = split * per, key_end = min(extent, key_first + per);
 
   // this lane's row
-  const int row = row0 + 32 * wave + c;
+  const int row = row0 + C * wave + c;
   const bool live = row < rows;
   const int tok = div_by(a.by_group, live ? row : last_row), head = kvh * a.G + (live ? row : last_row) - tok * a.G;
   const size_t qrow = (size_t)(a.start[s] + tok) * a.nh + head;
   const int lim = base + tok;  // the last visible position
   // of the wave's rows: no mask is needed up to wave_all, nothing is seen after wave_any
-  const int wrow = min(rows - 1, row0 + 32 * wave), wlast = min(rows - 1, row0 + 32 * wave + 31);
+  const int wrow = min(rows - 1, row0 + C * wave), wlast = min(rows - 1, row0 + C * wave + C - 1);
   const int wave_all = base + div_by(a.by_group, wrow), wave_any = base + div_by(a.by_group, wlast);
 
   v4u qv[KC];
@@ -551,174 +563,262 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, 
     const T *qp = (const T *)a.q + qrow * HD;
 #pragma unroll
     for (int i = 0; i < KC; i++)
-      qv[i] = live ? *(const v4u *)(qp + (32 / sizeof(T)) * i + (16 / sizeof(T)) * hf) : v4u{0, 0, 0, 0};
+      qv[i] = (live ? *(const v4u *)(qp + (16 / sizeof(T)) * (NG * i + g)) : v4u{0, 0, 0, 0}) ^ a.q_sign;
   }
-  v16f o[ND];
+  Acc o[ND];
 #pragma unroll
   for (int d = 0; d < ND; d++)
 #pragma unroll
-    for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-  float m_run = -INFINITY, l_run = 0.0f;
+    for (int i = 0; i < NA; i++) o[d][i] = 0.0f;
+  float m_ref = -INFINITY, l_run = 0.0f;  // the lane's own part of the sum
 
-  // this lane's part of a tile's copies: chunk and row of each of its NI pieces
+  // the XOR of a row: all 16 rows of a fragment in distinct banks, and the four rows
+  // that a transposing load takes together
+  auto swz = [](int r) { return CPR == 8 ? ((r & 2) << 1) | ((r >> 1) & 2) | ((r >> 3) & 1)
+                                              : ((r & 3) << 2) | ((r >> 1) & 2) | ((r >> 3) & 1); };
+  // This wave's part of a tile's copies: WR rows, this lane's 16-byte chunk of row
+  // u / CPR in each of NI pieces.  A tile's page ids are loaded two tiles ahead and
+  // looked at one tile ahead: a wait for them between would also wait for the copies.
+  // Absent positions and those behind key_end copy zeros (0 * NaN is NaN).
+  constexpr int WR = KT / Sh::kWaves;
   const unsigned lds0 = lds_addr(smem);
-  auto swz = [](int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; };
-  long long at[NI];
-  auto look_up = [&](int key0, int tag) {
-    bool bad = false;
+  auto swz_chunk = [&](int i) {  // source chunk of piece i
+    const int u = (wave * NI + i) * 64 + lane;
+    return (u % CPR) ^ swz(u / CPR);
+  };
+  int id[RUN ? 1 : NI];
+  auto load_ids = [&](int key0) {
+    if constexpr (RUN) {
+      const int p = key0 + wave * WR;
+      id[0] = p < key_end ? scalar_id(tab, div_by(a.map.div, p)) : -1;
+    } else {
 #pragma unroll
-    for (int i = 0; i < NI; i++) {
-      const int p = key0 + ((wave * NI + i) * 64 + lane) / CPR;
-      at[i] = p < key_end ? cell(a.map, tab, p) : -1;
-      bad |= p < key_end && at[i] < 0;
+      for (int i = 0; i < NI; i++) id[i] = tab[div_by(a.map.div, min(key0 + ((wave * NI + i) * 64 + lane) / CPR, key_end - 1))];
+    }
+  };
+  unsigned voff[RUN ? NI : 1];  // bytes from the run's first row
+  if constexpr (RUN) {
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+      voff[i] = (unsigned)((i * 64 + lane) / CPR) * (unsigned)a.map.row * (unsigned)sizeof(T) + 16 * swz_chunk(i);
+  }
+  auto copy = [&](int key0, int tag) {
+    const unsigned dst = lds0 + (tag & 1) * 2 * Sh::kTileBytes + wave * NI * 1024;
+    bool bad = false;
+    if constexpr (RUN) {
+      const int p = key0 + wave * WR, pg = div_by(a.map.div, p);
+      const bool there = (unsigned)id[0] < (unsigned)a.map.pages;
+      bad = p < key_end && !there;
+      const long long base = there ? (long long)id[0] * a.map.stride + (long long)(p - pg * a.map.page_size) * a.map.row : 0;
+      if (there && p + WR <= key_end) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+          dma_b128_s(kc + base, voff[i], dst + i * 1024);
+          dma_b128_s(vc + base, voff[i], dst + i * 1024 + Sh::kTileBytes);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+          const bool in = there && p + (i * 64 + lane) / CPR < key_end;
+          const char *z = (const char *)g_zero_row + 16 * swz_chunk(i);
+          dma_b128(in ? (const char *)(kc + base) + voff[i] : z, dst + i * 1024);
+          dma_b128(in ? (const char *)(vc + base) + voff[i] : z, dst + i * 1024 + Sh::kTileBytes);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const int p = key0 + ((wave * NI + i) * 64 + lane) / CPR, pg = div_by(a.map.div, p);
+        const bool there = (unsigned)id[i] < (unsigned)a.map.pages, in = there && p < key_end;
+        bad |= p < key_end && !there;
+        const long long at = (long long)id[i] * a.map.stride + (long long)(p - pg * a.map.page_size) * a.map.row;
+        const int ch = swz_chunk(i);
+        const char *z = (const char *)g_zero_row + 16 * ch;
+        dma_b128(in ? (const char *)(kc + at) + 16 * ch : z, dst + i * 1024);
+        dma_b128(in ? (const char *)(vc + at) + 16 * ch : z, dst + i * 1024 + Sh::kTileBytes);
+      }
     }
     if (__ballot(bad) && lane == 0) s_bad[tag & 3] = tag;
-  };
-  auto copy = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < NI; i++) {
-      const int u = (wave * NI + i) * 64 + lane, r = u / CPR, ch = (u % CPR) ^ swz(r);
-      const unsigned dst = lds0 + buf * 2 * Sh::kTileBytes + (wave * NI + i) * 1024;
-      const char *z = (const char *)g_zero_row + (16 * ch) % 1024;
-      dma_b128(at[i] >= 0 ? (const char *)(kc + at[i]) + 16 * ch : z, dst);
-      dma_b128(at[i] >= 0 ? (const char *)(vc + at[i]) + 16 * ch : z, dst + Sh::kTileBytes);
-    }
   };
 
   // Addresses within a tile, base ^ (chunk << 4) + row * RB: rows that differ by
   // 16 share their XOR, so a tile's reads have few distinct addresses and the rest
   // are immediate offsets.
-  const unsigned k_at = c * RB + ((hf ^ swz(c)) << 4);
-  const int vr0 = B16 ? 4 * hf + ((lane & 15) >> 2) : 4 * hf;
-  const unsigned v_at = B16 ? vr0 * RB + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swz(vr0)) << 4) + 8 * (lane & 1)
+  const unsigned k_at = c * RB + ((g ^ swz(c)) << 4);
+  const int vr0 = B16 ? 4 * g + ((lane & 15) >> 2) : 4 * g;
+  const unsigned v_at = B16 ? vr0 * RB + (((C == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1)) ^ swz(vr0)) * 16 + 8 * (lane & 1)
                             : vr0 * RB + (((c >> 2) ^ swz(vr0)) << 4) + 4 * (c & 3);
+  // the larger, or the sum, of a column's lane groups
+  auto over_groups = [&](float x, auto op) {
+    if constexpr (NG == 4) {
+      const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      x = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    }
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  };
 
   const int tiles = key_end > key_first ? (key_end - key_first + KT - 1) / KT : 0;
   if (tid < 4) s_bad[tid] = -1;
   __syncthreads();
   if (tiles > 0) {
-    look_up(key_first, 0);
-    copy(0);
-    if (tiles > 1) look_up(key_first + KT, 1);
+    load_ids(key_first);
+    copy(key_first, 0);
+    if (tiles > 1) load_ids(key_first + KT);
   }
   for (int it = 0; it < tiles; it++) {
     const int key0 = key_first + it * KT;
     wait_dma();
     __syncthreads();
     if (it + 1 < tiles) {
-      copy((it + 1) & 1);
-      if (it + 2 < tiles) look_up(key0 + 2 * KT, it + 2);
+      copy(key0 + KT, it + 1);
+      if (it + 2 < tiles) load_ids(key0 + 2 * KT);
     }
     if (key0 > wave_any) continue;
     const unsigned tile_at = lds0 + (it & 1) * 2 * Sh::kTileBytes;
     // formed anew for each tile: kept over the loop, they would fill the registers
     unsigned ka = k_at + tile_at, va = v_at + tile_at + Sh::kTileBytes;
     asm volatile("" : "+v"(ka), "+v"(va));
-    v16f sc[NS];
+    Acc sc[NS];
 #pragma unroll
     for (int b = 0; b < NS; b++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) sc[b][i] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < KC; i++)
-#pragma unroll
-      for (int b = 0; b < NS; b++) {
-        const v4u kf = lds_v4u((ka ^ (i << 5)) + 32 * b * RB);
-        if constexpr (B16) {
-          sc[b] = Mat16<T>::mul32(kf, qv[i], sc[b]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++) sc[b] = mfma_f32_32(__uint_as_float(kf[e]), __uint_as_float(qv[i][e]), sc[b]);
-          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-    // register i of subtile b: position key0 + 32 b + 8 (i / 4) + 4 hf + i % 4
+      for (int i = 0; i < NA; i++) sc[b][i] = 0.0f;
     const bool bad = s_bad[it & 3] == it;
+    // S^T, the fragments of the next GK chunks on their way while GK are multiplied;
+    // the fences keep the compiler from loading each where it is used
+    {
+      constexpr int GK = B16 ? (C == 16 ? 1 : 2) : 1, N = KC / GK;
+      v4u kf[2][GK][NS];
+      auto read = [&](int n) {
+#pragma unroll
+        for (int i = 0; i < GK; i++)
+#pragma unroll
+          for (int b = 0; b < NS; b++) kf[n & 1][i][b] = lds_v4u((ka ^ ((n * GK + i) * NG << 4)) + C * b * RB);
+      };
+      read(0);
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        if (n + 1 < N) read(n + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < GK; i++)
+#pragma unroll
+          for (int b = 0; b < NS; b++) {
+            if constexpr (!B16) {
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                sc[b] = mfma_f32_32(__uint_as_float(kf[n & 1][i][b][e]), __uint_as_float(qv[n * GK + i][e]), sc[b]);
+            } else if constexpr (C == 32) {
+              sc[b] = Mat16<T>::mul32(kf[n & 1][i][b], qv[n * GK + i], sc[b]);
+            } else {
+              sc[b] = Mat16<T>::mul16(kf[n & 1][i][b], qv[n * GK + i], sc[b]);
+            }
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
     if (key0 + KT - 1 > wave_all || key0 + KT > key_end || bad) {
+      unsigned long long present = ~0ull;
+      if (bad) present = __ballot(key0 + lane < key_end && lane < KT && cell(a.map, tab, min(key0 + lane, key_end - 1)) >= 0);
+      const int see = min(lim, key_end - 1) - key0;
 #pragma unroll
       for (int b = 0; b < NS; b++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int p = key0 + 32 * b + 8 * (i / 4) + 4 * hf + i % 4;
-          bool see = p <= lim && p < key_end;
-          if (bad && see) see = cell(a.map, tab, p) >= 0;
-          sc[b][i] = see ? sc[b][i] * a.scale : -INFINITY;
+        for (int i = 0; i < NA; i++) {
+          const int p = C * b + 4 * NG * (i / 4) + 4 * g + i % 4;
+          if (p > see || !(present >> p & 1)) sc[b][i] = -INFINITY;
         }
-    } else {
-#pragma unroll
-      for (int b = 0; b < NS; b++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) sc[b][i] *= a.scale;
     }
     float bm = sc[0][0];
 #pragma unroll
     for (int b = 0; b < NS; b++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[b][i]);
-    bm = fmaxf(bm, __shfl_xor(bm, 32));
-    const float m_new = fmaxf(m_run, bm), m_use = m_new == -INFINITY ? 0.0f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-    float ps = 0.0f;
-#pragma unroll
-    for (int b = 0; b < NS; b++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        sc[b][i] = __builtin_amdgcn_exp2f(sc[b][i] - m_use);
-        ps += sc[b][i];
-      }
-    ps += __shfl_xor(ps, 32);
-    l_run = __builtin_fmaf(l_run, alpha, ps);
-    if (__any(m_new != m_run)) {
+      for (int i = 0; i < NA; i++) bm = fmaxf(bm, sc[b][i]);
+    bm = over_groups(bm, [](float x, float y) { return fmaxf(x, y); }) * a.scale;
+    // any reference serves the softmax: it follows the maximum only when that has
+    // outgrown it by 2^8, so o is hardly ever rescaled
+    if (__any(bm > m_ref + 8.0f)) {
+      const float m_new = fmaxf(m_ref, bm), alpha = __builtin_amdgcn_exp2f(m_ref - (m_new == -INFINITY ? 0.0f : m_new));
+      m_ref = m_new;
+      l_run *= alpha;
 #pragma unroll
       for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] *= alpha;
+        for (int i = 0; i < NA; i++) o[d][i] *= alpha;
     }
-    m_run = m_new;
+    const float m_use = m_ref == -INFINITY ? 0.0f : m_ref;
+    float pr[KT / NG];  // in the order of the scores' registers
+#pragma unroll
+    for (int j = 0; j < KT / NG; j++) {
+      pr[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j / NA][j % NA], a.scale, -m_use));
+      l_run += pr[j];
+    }
     if constexpr (B16) {
-      constexpr int swz8 = CPR == 8 ? 4 : 8;  // swz of a row 8 further
+      // eight probabilities of a lane: positions 8 NG st + 4 NG q + 4 g + 0 .. 3
+      constexpr int swzq = C == 32 ? 1 : 0;                                  // what 4 NG rows further add to swz
+      constexpr int GV = C == 32 ? 2 : 4, N = KT / (8 * NG) * ND / GV;  // dim tiles of a group, groups
+      v2u vf[2][GV][2];
+      auto read = [&](int n) {
+        const int st = n / (ND / GV), d0 = n % (ND / GV) * GV;
 #pragma unroll
-      for (int st = 0; st < KT / 16; st++) {
-        const int b = st / 2, g = 8 * (st % 2);
-        const v4u pf = v4u{pack2<T>(sc[b][g], sc[b][g + 1]), pack2<T>(sc[b][g + 2], sc[b][g + 3]),
-                           pack2<T>(sc[b][g + 4], sc[b][g + 5]), pack2<T>(sc[b][g + 6], sc[b][g + 7])};
-#pragma unroll
-        for (int d = 0; d < ND; d++) {
-          v2u vf[2];
+        for (int d = 0; d < GV; d++)
 #pragma unroll
           for (int q = 0; q < 2; q++)
-            vf[q] = lds_transposed((va ^ (d << 6) ^ (q * swz8 << 4)) + (16 * st + 8 * q) * RB);
-          o[d] = Mat16<T>::mul32(v4u{vf[0][0], vf[0][1], vf[1][0], vf[1][1]}, pf, o[d]);
+            vf[n & 1][d][q] = lds_transposed((va ^ ((d0 + d) * (C / 8) << 4) ^ (q * swzq << 4)) + (8 * NG * st + 4 * NG * q) * RB);
+      };
+      read(0);
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        const int st = n / (ND / GV), d0 = n % (ND / GV) * GV;
+        if (n + 1 < N) read(n + 1);
+        const float *p8 = pr + 8 * st;
+        const v4u pf = v4u{pack2<T>(p8[0], p8[1]), pack2<T>(p8[2], p8[3]), pack2<T>(p8[4], p8[5]), pack2<T>(p8[6], p8[7])};
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < GV; d++) {
+          const v2u lo = vf[n & 1][d][0], hi = vf[n & 1][d][1];
+          const v4u vt = v4u{lo[0], lo[1], hi[0], hi[1]};
+          if constexpr (C == 32)
+            o[d0 + d] = Mat16<T>::mul32(vt, pf, o[d0 + d]);
+          else
+            o[d0 + d] = Mat16<T>::mul16(vt, pf, o[d0 + d]);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
+      float vf[2][ND];
+      auto read = [&](int i) {
         const int r = 8 * (i / 4) + i % 4;
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-          const float vf = lds_f32((va ^ (((8 * d) ^ (r & 15)) << 4)) + r * RB);
-          o[d] = mfma_f32_32(vf, sc[0][i], o[d]);
-        }
-        if (i % 2) __builtin_amdgcn_sched_barrier(0);
+        for (int d = 0; d < ND; d++) vf[i & 1][d] = lds_f32((va ^ (((8 * d) ^ swz(r)) << 4)) + r * RB);
+      };
+      read(0);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        if (i + 1 < 16) read(i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] = mfma_f32_32(vf[i & 1][d], pr[i], o[d]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
+  l_run = over_groups(l_run, [](float x, float y) { return x + y; });
   if (!live) return;
   if (a.po) {
     const size_t rec = ((size_t)split * a.rows + (a.start[s] - a.start[0] + tok)) * a.nh + head;
-    if (hf == 0) {
-      a.pm[rec] = m_run;
+    if (g == 0) {
+      a.pm[rec] = l_run == 0.0f ? -INFINITY : m_ref == -INFINITY ? 0.0f : m_ref;  // a NaN sum is kept
       a.pl[rec] = l_run;
     }
-    if (m_run == -INFINITY) return;
+    if (l_run == 0.0f) return;
     float *po = a.po + rec * HD;
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        *(v4f *)(po + 32 * d + 8 * i + 4 * hf) = v4f{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+      for (int i = 0; i < NA / 4; i++)
+        *(v4f *)(po + C * d + 4 * NG * i + 4 * g) = v4f{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
     return;
   }
   const float inv = l_run > 0.0f ? 1.0f / l_run : l_run == 0.0f ? 0.0f : l_run;
@@ -727,15 +827,15 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, 
 #pragma unroll
   for (int d = 0; d < ND; d++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int dim = 32 * d + 8 * i + 4 * hf;
+    for (int i = 0; i < NA / 4; i++) {
+      const int dim = C * d + 4 * NG * i + 4 * g;
       float y[4];
 #pragma unroll
       for (int e = 0; e < 4; e++) y[e] = o[d][4 * i + e] * inv;
       if (gp) {
-        const Pack<T, 4> g = *(const Pack<T, 4> *)(gp + dim);
+        const Pack<T, 4> gate = *(const Pack<T, 4> *)(gp + dim);
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] *= gate_sigmoid((float)g.v[e]);
+        for (int e = 0; e < 4; e++) y[e] *= gate_sigmoid((float)gate.v[e]);
       }
       Pack<T, 4> r;
 #pragma unroll
@@ -842,14 +942,20 @@ void launch_join(const JoinArgs &a, int hd, int rows, hipStream_t st) {
 }
 
 constexpr int kPromptRows = 128;
-template <class T, int HD>
+template <class T, int HD, bool RUN>
 int launch_prompt(const char *name, const PromptArgs &a, dim3 grid, hipStream_t st) {
   typedef PromptShape<T, HD> Sh;
   const hipError_t e =
-      hipFuncSetAttribute((const void *)k_paged_prompt<T, HD>, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds);
+      hipFuncSetAttribute((const void *)k_paged_prompt<T, HD, RUN>, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds);
   if (e != hipSuccess) return fail_hip(name, e);
-  k_paged_prompt<T, HD><<<grid, 64 * Sh::kWaves, Sh::kLds, st>>>(a);
+  k_paged_prompt<T, HD, RUN><<<grid, 64 * Sh::kWaves, Sh::kLds, st>>>(a);
   return 0;
+}
+template <class T, int HD>
+int launch_prompt(const char *name, const PromptArgs &a, dim3 grid, hipStream_t st) {
+  typedef PromptShape<T, HD> Sh;
+  return a.map.page_size % (Sh::kKeys / Sh::kWaves) == 0 ? launch_prompt<T, HD, true>(name, a, grid, st)
+                                                         : launch_prompt<T, HD, false>(name, a, grid, st);
 }
 static_assert(PromptShape<float, 64>::kRows == kPromptRows && PromptShape<__bf16, 256>::kRows == kPromptRows, "rows of a tile");
 template <class T>
@@ -1036,7 +1142,9 @@ extern "C" int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *c, void *o
   a.gate_stride = gate_stride;
   a.gate_head = gate_head_stride;
   a.nh = nh, a.nkv = c->kv_heads, a.G = G;
-  a.scale = scale * kLog2e;
+  a.scale = fabsf(scale) * kLog2e;
+  if (!(a.scale >= 1e-38f)) a.scale = 1e-38f;  // no scores at all: equal ones
+  if (scale < 0.0f) a.q_sign = c->type == COLI_TYPE_F32 ? 0x80000000u : 0x80008000u;
   a.by_group = fast_div(G);
   a.map = page_map(c, table);
   for (int s0 = 0; s0 < sequences; s0 += kSeqs) {
