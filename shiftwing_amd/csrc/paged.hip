@@ -463,7 +463,7 @@ struct PromptArgs {
   int gate_head, nh, nkv, G, seqs, first_seq, splits, rows;
   float scale;      // |scale| * log2(e)
   unsigned q_sign;  // sign bits of a register of queries where scale is negative
-  FastDiv by_group;
+  FastDiv by_group, by_heads;  // by G, by nkv
   PageMap map;
   int start[kSeqs + 1], len[kSeqs], tile0[kSeqs + 1];  // sequence s's tiles are tile0[s] .. tile0[s + 1] - 1
 };
@@ -515,6 +515,51 @@ struct PromptShape {
 // (16 bits) or as single values (fp32).
 // LDS rows are stored with their 16-byte chunks exchanged by an XOR with the row
 // number, which spreads every access over all banks.
+// the XOR of a row of CPR chunks.  Bit by bit a sum of row bits, so that rows which
+// differ by a constant differ by a constant here too; chosen so that 16 rows of a
+// fragment of 32 or 16 columns, taken in the hardware's groups of 16 lanes, and the
+// rows that a transposing load takes together lie in distinct banks.
+template <int CPR>
+__host__ __device__ constexpr int chunk_xor(int r) {
+  return CPR == 8 ? ((r & 2) << 1) | ((r >> 1) & 2) | ((r >> 3) & 1)
+                  : ((r & 3) << 2) | (((r >> 1) ^ (r >> 2)) & 2) | ((r >> 3) & 1);
+}
+
+// Tile x of a launch, heavy ones first: tiles by their number within their sequence
+// (later ones see more), the sequences' last ones first.  Tile number l is preceded by
+// count(l + 1) tiles, count(l) = sum over sequences of max(0, tiles - l).
+__device__ __forceinline__ void pick_tile(const int *tile0, int seqs, int x, int &seq, int &tile) {
+  if (seqs == 1) {
+    seq = 0;
+    tile = tile0[1] - 1 - x;
+    return;
+  }
+  static_assert(kSeqs == 128, "two sequences a lane");
+  const int lane = threadIdx.x & 63;
+  const int n0 = lane < seqs ? tile0[lane + 1] - tile0[lane] : 0;
+  const int n1 = lane + 64 < seqs ? tile0[lane + 65] - tile0[lane + 64] : 0;
+  auto count = [&](int l) { return wave_sum_dpp(max(0, n0 - l) + max(0, n1 - l)); };
+  int lo = 0, hi = (int)wave_max_u32((unsigned)max(n0, n1));  // count(lo) > x >= count(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (count(mid) <= x)
+      hi = mid;
+    else
+      lo = mid;
+  }
+  tile = hi - 1;
+  int rank = x - count(hi);
+  unsigned long long have = __ballot(n0 >= hi);
+  seq = 0;
+  if (rank >= __builtin_popcountll(have)) {
+    rank -= __builtin_popcountll(have);
+    have = __ballot(n1 >= hi);
+    seq = 64;
+  }
+  const unsigned long long below = have & ((1ull << lane) - 1);
+  seq += __builtin_ctzll(__ballot((have >> lane & 1) && __builtin_popcountll(below) == rank));
+}
+
 // RUN: pages hold whole runs of the WR positions that a wave copies, whose page is
 // then looked up once, by a scalar load.
 template <class T, int HD, bool RUN>
@@ -532,12 +577,12 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, 
   int *s_bad = (int *)(smem + 4 * Sh::kTileBytes);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & (C - 1),
             g = lane / C;
-  const int kvh = blockIdx.y, split = blockIdx.z;
-  // late tiles see most and go first
-  const int tile = gridDim.x - 1 - blockIdx.x;
-  const int s = find_span(a.tile0, a.seqs, tile);
+  // kv heads in turn, so that each die, which gets every eighth workgroup, has few
+  const int x = div_by(a.by_heads, blockIdx.x), kvh = blockIdx.x - x * a.nkv, split = blockIdx.z;
+  int s, tile;
+  pick_tile(a.tile0, a.seqs, x, s, tile);
   const int rows = (a.start[s + 1] - a.start[s]) * a.G;        // of the sequence and kv head
-  const int row0 = (tile - a.tile0[s]) * Sh::kRows;
+  const int row0 = tile * Sh::kRows;
   const int base = a.len[s] - (a.start[s + 1] - a.start[s]);  // positions before the first row
   const int *tab = a.map.table + (size_t)(a.first_seq + s) * a.map.table_pages;
   const T *kc = (const T *)a.k + (size_t)kvh * HD, *vc = (const T *)a.v + (size_t)kvh * HD;
@@ -572,10 +617,6 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, 
     for (int i = 0; i < NA; i++) o[d][i] = 0.0f;
   float m_ref = -INFINITY, l_run = 0.0f;  // the lane's own part of the sum
 
-  // the XOR of a row: all 16 rows of a fragment in distinct banks, and the four rows
-  // that a transposing load takes together
-  auto swz = [](int r) { return CPR == 8 ? ((r & 2) << 1) | ((r >> 1) & 2) | ((r >> 3) & 1)
-                                              : ((r & 3) << 2) | ((r >> 1) & 2) | ((r >> 3) & 1); };
   // This wave's part of a tile's copies: WR rows, this lane's 16-byte chunk of row
   // u / CPR in each of NI pieces.  A tile's page ids are loaded two tiles ahead and
   // looked at one tile ahead: a wait for them between would also wait for the copies.
@@ -584,7 +625,7 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, 
   const unsigned lds0 = lds_addr(smem);
   auto swz_chunk = [&](int i) {  // source chunk of piece i
     const int u = (wave * NI + i) * 64 + lane;
-    return (u % CPR) ^ swz(u / CPR);
+    return (u % CPR) ^ chunk_xor<CPR>(u / CPR);
   };
   int id[RUN ? 1 : NI];
   auto load_ids = [&](int key0) {
@@ -644,10 +685,10 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, 
   // Addresses within a tile, base ^ (chunk << 4) + row * RB: rows that differ by
   // 16 share their XOR, so a tile's reads have few distinct addresses and the rest
   // are immediate offsets.
-  const unsigned k_at = c * RB + ((g ^ swz(c)) << 4);
+  const unsigned k_at = c * RB + ((g ^ chunk_xor<CPR>(c)) << 4);
   const int vr0 = B16 ? 4 * g + ((lane & 15) >> 2) : 4 * g;
-  const unsigned v_at = B16 ? vr0 * RB + (((C == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1)) ^ swz(vr0)) * 16 + 8 * (lane & 1)
-                            : vr0 * RB + (((c >> 2) ^ swz(vr0)) << 4) + 4 * (c & 3);
+  const unsigned v_at = B16 ? vr0 * RB + (((C == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1)) ^ chunk_xor<CPR>(vr0)) * 16 + 8 * (lane & 1)
+                            : vr0 * RB + (((c >> 2) ^ chunk_xor<CPR>(vr0)) << 4) + 4 * (c & 3);
   // the larger, or the sum, of a column's lane groups
   auto over_groups = [&](float x, auto op) {
     if constexpr (NG == 4) {
@@ -756,7 +797,7 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, 
     }
     if constexpr (B16) {
       // eight probabilities of a lane: positions 8 NG st + 4 NG q + 4 g + 0 .. 3
-      constexpr int swzq = C == 32 ? 1 : 0;                                  // what 4 NG rows further add to swz
+      constexpr int swzq = chunk_xor<CPR>(4 * NG);
       constexpr int GV = C == 32 ? 2 : 4, N = KT / (8 * NG) * ND / GV;  // dim tiles of a group, groups
       v2u vf[2][GV][2];
       auto read = [&](int n) {
@@ -791,7 +832,7 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, 
       auto read = [&](int i) {
         const int r = 8 * (i / 4) + i % 4;
 #pragma unroll
-        for (int d = 0; d < ND; d++) vf[i & 1][d] = lds_f32((va ^ (((8 * d) ^ swz(r)) << 4)) + r * RB);
+        for (int d = 0; d < ND; d++) vf[i & 1][d] = lds_f32((va ^ (((8 * d) ^ chunk_xor<CPR>(r)) << 4)) + r * RB);
       };
       read(0);
 #pragma unroll
@@ -1146,6 +1187,7 @@ extern "C" int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *c, void *o
   if (!(a.scale >= 1e-38f)) a.scale = 1e-38f;  // no scores at all: equal ones
   if (scale < 0.0f) a.q_sign = c->type == COLI_TYPE_F32 ? 0x80000000u : 0x80008000u;
   a.by_group = fast_div(G);
+  a.by_heads = fast_div(c->kv_heads);
   a.map = page_map(c, table);
   for (int s0 = 0; s0 < sequences; s0 += kSeqs) {
     const int n = sequences - s0 < kSeqs ? sequences - s0 : kSeqs, rows = start[s0 + n] - start[s0];
@@ -1156,7 +1198,7 @@ extern "C" int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *c, void *o
     for (int s = 0; s < n; s++) {
       const int m = start[s0 + s + 1] - start[s0 + s];
       tiles += ((long long)m * G + R - 1) / R;
-      if (tiles > INT_MAX) return fail_arg("%s: too many rows", name);
+      if (tiles * c->kv_heads > INT_MAX) return fail_arg("%s: too many rows", name);
       a.tile0[s + 1] = (int)tiles;
       if (m && length[s0 + s] > longest) longest = length[s0 + s];
     }
@@ -1172,7 +1214,7 @@ extern "C" int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *c, void *o
     a.splits = splits < 1 ? 1 : (int)splits;
     a.po = a.pm = a.pl = nullptr;
     if (a.splits > 1 && partials(ctx, name, (size_t)a.splits * rows, nh, hd, &a.po, &a.pm, &a.pl)) return -1;
-    const dim3 grid((unsigned)tiles, c->kv_heads, a.splits);
+    const dim3 grid((unsigned)(tiles * c->kv_heads), 1, a.splits);
     const int rc = c->type == COLI_TYPE_F32   ? launch_prompt<float>(name, a, hd, grid, ctx->stream)
                    : c->type == COLI_TYPE_F16 ? launch_prompt<_Float16>(name, a, hd, grid, ctx->stream)
                                               : launch_prompt<__bf16>(name, a, hd, grid, ctx->stream);
