@@ -467,9 +467,6 @@ struct ScanLds {
   static constexpr int kD = kS;                                 // d lies where the state was
   static constexpr int kX = kS + 3 * kState, kR = kX + 3 * kTok, kAll = kR + 3 * kTok;
 };
-// A barrier that waits for this wave's LDS accesses alone: __syncthreads would also
-// wait for the next chunk's loads in flight.
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Wint-to-pointer-cast"
 typedef short v4s __attribute__((ext_vector_type(4)));

@@ -159,17 +159,25 @@ __device__ __forceinline__ v4f mfma_f32_16(float a, float b, v4f c) {
 // One workgroup of 4 waves a (sequence, split of its positions, kv head, group of
 // 16 query heads); a wave takes every fourth block of KB positions.  The scores
 // come transposed, S^T (positions x heads) = K Q^T, so that a lane holds one head's
-// probabilities of the positions 4 kg + i whose values it also loads: the second
+// probabilities of the positions 4 kg + j whose values it also loads: the second
 // product O^T (dims x heads) += V^T P^T takes them as they are.  Its A operand wants
 // consecutive positions of one dim where memory has consecutive dims of one
 // position: in 16 bits a lane loads 8 dims of 8 positions and regroups them by byte
 // permutes (16 to 16 loaded registers), an fp32 lane's value is the operand itself;
 // row n of dim tile d stands for dim W n + d (tiles of one load).
-// Nothing goes through LDS until the waves' merge.  HBM-bound.
+// Nothing goes through LDS until the waves' merge.  HBM-bound: a block's keys are
+// loaded as soon as the last ones' registers are free, its values likewise, so that a
+// wave always has one of them in flight.
 // RUN16: pages hold whole runs of 16 positions, whose page the wave then looks up
-// once, by a scalar load; otherwise every lane looks up its own positions.
+// once, by a scalar load, a block ahead; otherwise every lane looks up its own.
+template <class T, int HD>
+struct DecodeShape {
+  static constexpr bool B16 = sizeof(T) == 2;
+  static constexpr int kPerCu = HD == 64 ? 3 : HD == 128 ? 2 : 1;  // workgroups of a compute unit, by their registers
+  static constexpr int kLeast = 4 * (B16 ? 32 : 16);               // positions of a split: one block a wave
+};
 template <class T, int HD, bool RUN16>
-__global__ __launch_bounds__(256) void k_paged_decode(DecodeArgs a) {
+__global__ __launch_bounds__(256, (DecodeShape<T, HD>::kPerCu)) void k_paged_decode(DecodeArgs a) {
   constexpr bool B16 = sizeof(T) == 2;
   constexpr int NB = B16 ? 2 : 1, KB = 16 * NB;            // runs and positions of a block
   constexpr int NT = HD / 16;                              // dim tiles
@@ -177,10 +185,11 @@ __global__ __launch_bounds__(256) void k_paged_decode(DecodeArgs a) {
   constexpr int W = B16 ? (HD >= 128 ? 8 : 4) : 4;         // values of one load
   constexpr int NW = NT / W;                               // loads of one position
   constexpr int LV = W * (int)sizeof(T) / 4;               // registers of one load
-  __shared__ float s_m[4][16], s_l[4][16], s_lsum[16];
-  __shared__ float s_o[16 * (HD + 1)];
-  __shared__ v4u s_q[B16 ? 1 : KR * 64];                   // fp32: [chunk][lane]
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  typedef unsigned VL __attribute__((ext_vector_type(LV)));
+  constexpr int OP = HD + 4;                               // pitch of a head's outputs in LDS
+  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ __align__(16) float s_o[4][16 * OP];          // fp32: the queries first, [chunk][lane] x 16 bytes
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
   const int per_split = a.nkv * a.hgroups;
   const int slot = blockIdx.x / per_split, sub = blockIdx.x % per_split;
   const int kvh = sub / a.hgroups, hg = sub % a.hgroups;
@@ -191,93 +200,100 @@ __global__ __launch_bounds__(256) void k_paged_decode(DecodeArgs a) {
   const int *tab = a.map.table + (size_t)(a.first_seq + r) * a.map.table_pages;
   const T *kc = (const T *)a.k + (size_t)kvh * HD, *vc = (const T *)a.v + (size_t)kvh * HD;
 
-  // the queries: B operand of the first product; heads beyond the group are zero
-  v4u qv[B16 ? KR : 1];
+  // where the positions of a block lie: a run's first cell, or this lane's cells (of
+  // key n, of the values 4 kg + j); -1 where there is none
+  struct Loc {
+    int id[NB];                        // RUN16: the runs' page ids
+    long long k[NB], v[NB][RUN16 ? 1 : 4];
+  };
+  auto look_up = [&](Loc &l, int key0) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      const int p0 = key0 + 16 * b;
+      if constexpr (RUN16) {
+        l.id[b] = p0 < key_end ? scalar_id(tab, div_by(a.map.div, p0)) : -1;
+      } else {
+        l.k[b] = p0 + n < key_end ? cell(a.map, tab, p0 + n) : -1;
+#pragma unroll
+        for (int j = 0; j < 4; j++) l.v[b][j] = p0 + 4 * kg + j < key_end ? cell(a.map, tab, p0 + 4 * kg + j) : -1;
+      }
+    }
+  };
+  auto find_runs = [&](Loc &l, int key0) {  // RUN16: the ids have come
+    if constexpr (RUN16)
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        const int p0 = key0 + 16 * b, pg = div_by(a.map.div, p0);
+        l.k[b] = (unsigned)l.id[b] < (unsigned)a.map.pages
+                     ? (long long)l.id[b] * a.map.stride + (long long)(p0 - pg * a.map.page_size) * a.map.row
+                     : -1;
+      }
+  };
+  // a position that is not there reads another cell of the pool and is masked below
+  v4u kr[NB][KR];
+  VL vr[NB][4][NW];
+  auto load_keys = [&](const Loc &l, int key0) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      const T *kp;
+      if constexpr (RUN16)
+        kp = kc + (l.k[b] >= 0 ? l.k[b] : 0) + (unsigned)max(0, min(n, key_end - 1 - key0 - 16 * b)) * (unsigned)a.map.row;
+      else
+        kp = kc + (l.k[b] >= 0 ? l.k[b] : 0);
+#pragma unroll
+      for (int i = 0; i < KR; i++) kr[b][i] = *(const v4u *)(kp + (64 / sizeof(T)) * i + (16 / sizeof(T)) * kg);
+    }
+  };
+  auto load_values = [&](const Loc &l, int key0) {
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const T *vp;
+        if constexpr (RUN16)
+          vp = vc + (l.k[b] >= 0 ? l.k[b] : 0) +
+               (unsigned)max(0, min(4 * kg + j, key_end - 1 - key0 - 16 * b)) * (unsigned)a.map.row;
+        else
+          vp = vc + (l.v[b][j] >= 0 ? l.v[b][j] : 0);
+        vp += W * n;
+#pragma unroll
+        for (int w = 0; w < NW; w++) vr[b][j][w] = *(const VL *)(vp + 16 * W * w);
+      }
+  };
+
+  // the queries, B operand of the first product (fp32 ones by way of LDS; heads beyond
+  // the group are zero), go out before the first block: loads come back in order
+  constexpr int QR = B16 ? KR : KR / 4;
+  v4u qv[QR];
   {
     const T *qrow = (const T *)a.q + ((size_t)r * a.nh + h0 + n) * HD;
-    if constexpr (B16) {
 #pragma unroll
-      for (int i = 0; i < KR; i++) qv[i] = n < heads ? *(const v4u *)(qrow + 32 * i + 8 * kg) : v4u{0, 0, 0, 0};
-    } else {
-      for (int i = wave; i < KR; i += 4)
-        s_q[i * 64 + lane] = n < heads ? *(const v4u *)(qrow + 16 * i + 4 * kg) : v4u{0, 0, 0, 0};
-      __syncthreads();
-    }
+    for (int i = 0; i < QR; i++)
+      qv[i] = n < heads ? *(const v4u *)(qrow + (64 / sizeof(T)) * (B16 ? i : 4 * i + wave) + (16 / sizeof(T)) * kg) : v4u{0, 0, 0, 0};
+  }
+  int key0 = key_first + wave * KB;
+  Loc cur, nxt;
+  if (key0 < key_end) {
+    look_up(cur, key0);
+    find_runs(cur, key0);
+    load_keys(cur, key0);
+    load_values(cur, key0);
+  }
+  if constexpr (!B16) {
+#pragma unroll
+    for (int i = 0; i < QR; i++) ((v4u *)s_o)[(4 * i + wave) * 64 + lane] = qv[i];
+    lds_barrier();
   }
   v4f o[NT];
 #pragma unroll
   for (int d = 0; d < NT; d++) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
   float m_run = -INFINITY, l_run = 0.0f;
 
-  for (int key0 = key_first + wave * KB; key0 < key_end; key0 += 4 * KB) {
-    // keys 16 b + n (A operand) and values of positions 16 b + 4 kg + j; a position
-    // that is not there reads the first cell of the pool and is masked below
-    v4u kr[NB][KR];
-    unsigned vr[NB][4][NW][LV];
-    bool there[NB][4];
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      const int p0 = key0 + 16 * b;
-      long long base = -1;
-      if (RUN16) {
-        const int u0 = __builtin_amdgcn_readfirstlane(p0);
-        if (u0 < key_end) base = cell(a.map, tab, u0);
-      }
-      long long ck, cv[4];
-      if (RUN16) {
-        ck = base >= 0 && p0 + n < key_end ? base + (long long)n * a.map.row : -1;
-      } else {
-        ck = p0 + n < key_end ? cell(a.map, tab, p0 + n) : -1;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int p = p0 + 4 * kg + j;
-        if (RUN16)
-          cv[j] = base >= 0 && p < key_end ? base + (long long)(4 * kg + j) * a.map.row : -1;
-        else
-          cv[j] = p < key_end ? cell(a.map, tab, p) : -1;
-        there[b][j] = cv[j] >= 0;
-      }
-      const T *kp = kc + (ck >= 0 ? ck : 0);
-#pragma unroll
-      for (int i = 0; i < KR; i++) kr[b][i] = *(const v4u *)(kp + (64 / sizeof(T)) * i + (16 / sizeof(T)) * kg);
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const T *vp = vc + (cv[j] >= 0 ? cv[j] : 0) + W * n;
-#pragma unroll
-        for (int w = 0; w < NW; w++) {
-          if constexpr (LV == 4) {
-            const v4u x = *(const v4u *)(vp + 16 * W * w);
-#pragma unroll
-            for (int e = 0; e < 4; e++) vr[b][j][w][e] = x[e];
-          } else {
-            const v2u x = *(const v2u *)(vp + 16 * W * w);
-            vr[b][j][w][0] = x[0];
-            vr[b][j][w][1] = x[1];
-          }
-        }
-      }
-    }
-    // every load of the block is in flight before the first product
-    asm volatile("" ::: "memory");
-    // values behind the end may be anything (0 * NaN is NaN): they become zero
-    bool whole = true;
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) whole &= there[b][j];
-    if (!__all(whole)) {
-#pragma unroll
-      for (int b = 0; b < NB; b++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-          for (int w = 0; w < NW; w++)
-#pragma unroll
-            for (int e = 0; e < LV; e++) vr[b][j][w][e] = there[b][j] ? vr[b][j][w][e] : 0u;
-    }
+  if (key0 < key_end) for (;;) {
+    const int next0 = key0 + 4 * KB;
+    const bool more = next0 < key_end;
+    if (more) look_up(nxt, next0);
     float sv[NB][4];
-    float bm = -INFINITY;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
       v4f sc;
@@ -293,23 +309,49 @@ __global__ __launch_bounds__(256) void k_paged_decode(DecodeArgs a) {
         v4f c[4] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int i = 0; i < KR; i++) {
-          const v4u qq = s_q[i * 64 + lane];
+          const v4u qq = ((const v4u *)s_o)[i * 64 + lane];
 #pragma unroll
           for (int e = 0; e < 4; e++) c[e] = mfma_f32_16(__uint_as_float(kr[b][i][e]), __uint_as_float(qq[e]), c[e]);
         }
         sc = (c[0] + c[1]) + (c[2] + c[3]);
       }
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        sv[b][j] = there[b][j] ? sc[j] * a.scale : -INFINITY;
-        bm = fmaxf(bm, sv[b][j]);
-      }
+      for (int j = 0; j < 4; j++) sv[b][j] = sc[j] * a.scale;
     }
+    if (more) {
+      find_runs(nxt, next0);
+      load_keys(nxt, next0);
+    }
+    // positions behind the end or without a page: no score, and a zero value (what lies
+    // there may be anything, and 0 * NaN is NaN)
+    bool there[NB][4], whole = true;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        there[b][j] = RUN16 ? cur.k[b] >= 0 && key0 + 16 * b + 4 * kg + j < key_end : cur.v[b][RUN16 ? 0 : j] >= 0;
+        whole &= there[b][j];
+      }
+    if (!__all(whole)) {
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          sv[b][j] = there[b][j] ? sv[b][j] : -INFINITY;
+#pragma unroll
+          for (int w = 0; w < NW; w++) vr[b][j][w] = there[b][j] ? vr[b][j][w] : VL(0u);
+        }
+    }
+    float bm = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) bm = fmaxf(bm, sv[b][j]);
     bm = fmaxf(bm, __shfl_xor(bm, 16));
     bm = fmaxf(bm, __shfl_xor(bm, 32));
     const float m_new = fmaxf(m_run, bm), m_use = m_new == -INFINITY ? 0.0f : m_new;
     const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-    float ps = 0.0f;
+    float ps = 0.0f;  // this lane's positions; the lanes of a head meet at the end
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -317,8 +359,6 @@ __global__ __launch_bounds__(256) void k_paged_decode(DecodeArgs a) {
         sv[b][j] = __builtin_amdgcn_exp2f(sv[b][j] - m_use);
         ps += sv[b][j];
       }
-    ps += __shfl_xor(ps, 16);
-    ps += __shfl_xor(ps, 32);
     l_run = __builtin_fmaf(l_run, alpha, ps);
     m_run = m_new;
 #pragma unroll
@@ -344,57 +384,67 @@ __global__ __launch_bounds__(256) void k_paged_decode(DecodeArgs a) {
 #pragma unroll
         for (int d = 0; d < NT; d++) o[d] = mfma_f32_16(__uint_as_float(vr[0][j][d / W][d % W]), sv[0][j], o[d]);
     }
+    if (!more) break;
+    load_values(nxt, next0);
+    cur = nxt;
+    key0 = next0;
   }
 
-  // the waves meet in LDS, in wave order
+  // the waves meet in LDS, summed in wave order
+  l_run += __shfl_xor(l_run, 16);
+  l_run += __shfl_xor(l_run, 32);
   if (kg == 0) {
     s_m[wave][n] = m_run;
     s_l[wave][n] = l_run;
   }
+  if (!B16) __syncthreads();  // the queries have been read
+#pragma unroll
+  for (int d = 0; d < NT; d += 4)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      *(v4f *)(s_o[wave] + n * OP + 16 * W * (d / W) + W * (4 * kg + i) + d % W) = v4f{o[d][i], o[d + 1][i], o[d + 2][i], o[d + 3][i]};
   __syncthreads();
-  float M = s_m[0][n];
-#pragma unroll
-  for (int w = 1; w < 4; w++) M = fmaxf(M, s_m[w][n]);
-  const float f = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - M);
-  for (int w = 0; w < 4; w++) {
-    if (wave == w) {
-#pragma unroll
-      for (int d = 0; d < NT; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float *p = s_o + (size_t)n * (HD + 1) + 16 * W * (d / W) + W * (4 * kg + i) + d % W;
-          *p = w == 0 ? o[d][i] * f : __builtin_fmaf(o[d][i], f, *p);
-        }
-    }
-    __syncthreads();
-  }
-  if (threadIdx.x < 16) {
+  auto total = [&](int h, float &M, float (&f)[4]) {  // largest score, sum, and the waves' weights
+    M = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
     float L = 0.0f;
-    for (int w = 0; w < 4; w++)
-      if (s_m[w][n] != -INFINITY) L = __builtin_fmaf(s_l[w][n], __builtin_amdgcn_exp2f(s_m[w][n] - M), L);
-    s_lsum[n] = L;
-    if (a.po && n < heads) {
-      a.pm[(size_t)slot * a.nh + h0 + n] = M;
-      a.pl[(size_t)slot * a.nh + h0 + n] = L;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      f[w] = s_m[w][h] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[w][h] - M);
+      // a wave without a visible position has sums of zero; a NaN sum is kept
+      L = __builtin_fmaf(s_l[w][h], s_m[w][h] == -INFINITY ? 1.0f : f[w], L);
     }
+    return L;
+  };
+  if (a.po && threadIdx.x < heads) {
+    float M, f[4];
+    const float L = total(threadIdx.x, M, f);
+    a.pm[(size_t)slot * a.nh + h0 + threadIdx.x] = L == 0.0f ? -INFINITY : M == -INFINITY ? 0.0f : M;
+    a.pl[(size_t)slot * a.nh + h0 + threadIdx.x] = L;
   }
-  __syncthreads();
-  for (int u = threadIdx.x; u < heads * HD; u += 256) {
-    const int h = u / HD, d = u % HD;
-    const float x = s_o[h * (HD + 1) + d];
+  for (int u = threadIdx.x; u < heads * HD / 4; u += 256) {
+    const int h = u / (HD / 4), d = u % (HD / 4) * 4;
+    float M, f[4];
+    const float L = total(h, M, f);
+    v4f x = *(const v4f *)(s_o[0] + h * OP + d) * f[0];
+#pragma unroll
+    for (int w = 1; w < 4; w++) x += *(const v4f *)(s_o[w] + h * OP + d) * f[w];
     if (a.po) {
-      a.po[((size_t)slot * a.nh + h0 + h) * HD + d] = x;
+      *(v4f *)(a.po + ((size_t)slot * a.nh + h0 + h) * HD + d) = x;
       continue;
     }
-    float y = s_lsum[h] > 0.0f ? x / s_lsum[h] : s_lsum[h] == 0.0f ? 0.0f : s_lsum[h];  // NaN stays
-    if (a.gate) y *= gate_sigmoid((float)((const T *)a.gate)[(size_t)r * a.gate_stride + (size_t)(h0 + h) * a.gate_head + d]);
-    ((T *)a.out)[((size_t)r * a.nh + h0 + h) * HD + d] = (T)y;
+    const float inv = L > 0.0f ? 1.0f / L : L;  // 0 stays, and a NaN
+    Pack<T, 4> y, g;
+    if (a.gate) g = *(const Pack<T, 4> *)((const T *)a.gate + (size_t)r * a.gate_stride + (size_t)(h0 + h) * a.gate_head + d);
+#pragma unroll
+    for (int e = 0; e < 4; e++) y.v[e] = (T)(x[e] * inv * (a.gate ? gate_sigmoid((float)g.v[e]) : 1.0f));
+    *(Pack<T, 4> *)((T *)a.out + ((size_t)r * a.nh + h0 + h) * HD + d) = y;
   }
 }
 
-// Joins the splits of one (row, query head): the weights 2^(m - M) in LDS, then
-// 256 / HD groups of threads sum every NG-th split, eight loads in flight, and
-// meet in LDS in group order.  grid (query heads, rows), S <= kMaxSplits.
+// Joins the splits of one (row, query head): the weights 2^(m - M) in LDS, while the
+// first outputs are on their way; a thread has four dims of every NG-th split, eight
+// loads in flight, and the groups meet in LDS in their order.
+// grid (query heads, rows), 512 threads, S <= kMaxSplits.
 constexpr int kMaxSplits = 256;
 struct JoinArgs {
   const float *po, *pm, *pl;
@@ -407,38 +457,49 @@ struct JoinArgs {
   int first[kSeqs + 1];  // flat: row r's records
 };
 template <class T, int HD>
-__global__ __launch_bounds__(256) void k_paged_join(JoinArgs a) {
-  constexpr int NG = 256 / HD;
-  __shared__ float s_w[kMaxSplits], s_red[8], s_o[NG][HD];
+__global__ __launch_bounds__(512) void k_paged_join(JoinArgs a) {
+  constexpr int TH = HD / 4, NG = 512 / TH, B = 8;
+  __shared__ float s_w[kMaxSplits], s_red[16];
+  __shared__ v4f s_o[NG][TH];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = blockIdx.x, t = blockIdx.y;
   const int S = a.flat ? a.first[t + 1] - a.first[t] : a.S;
   const size_t base = a.flat ? (size_t)a.first[t] : (size_t)t, step = a.flat ? 1 : (size_t)a.step;
+  const int d = tid % TH, g = tid / TH;
+  const float *po = a.po + (base * a.nh + h) * HD + 4 * d;
+  const size_t pitch = step * a.nh * HD;
+  v4f x[B];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < B; k++) {
+      const int s = s0 + k * NG;
+      x[k] = *(const v4f *)(po + (s < S ? s : 0) * pitch);
+    }
+  };
+  load(g);
   const size_t rec = ((base + (size_t)(tid < S ? tid : 0) * step) * a.nh) + h;
   const float m = tid < S ? a.pm[rec] : -INFINITY, lv = tid < S ? a.pl[rec] : 0.0f;
   const float wm = wave_max_dpp(m);
   if (lane == 0) s_red[wave] = wm;
   __syncthreads();
-  const float M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  float M = s_red[0];
+#pragma unroll
+  for (int w = 1; w < 8; w++) M = fmaxf(M, s_red[w]);
   const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-  s_w[tid] = w;
+  if (tid < kMaxSplits) s_w[tid] = w;
   const float ls = wave_sum_dpp(w == 0.0f ? 0.0f : lv * w);
-  if (lane == 0) s_red[4 + wave] = ls;
+  if (lane == 0) s_red[8 + wave] = ls;
   __syncthreads();
-  const float L = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
-  const int d = tid % HD, g = tid / HD;
-  float o = 0.0f;
-  for (int s0 = g; s0 < S; s0 += 8 * NG) {
-    float x[8];
+  float L = s_red[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-      const int s = s0 + k * NG;
-      x[k] = a.po[((base + (size_t)(s < S ? s : g) * step) * a.nh + h) * HD + d];
-    }
+  for (int k = 1; k < 8; k++) L += s_red[8 + k];
+  v4f o = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = g; s0 < S; s0 += B * NG) {
+    if (s0 != g) load(s0);
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
+    for (int k = 0; k < B; k++) {
       const int s = s0 + k * NG;
       // a record without a visible position holds nothing
-      if (s < S && s_w[s] != 0.0f) o = __builtin_fmaf(x[k], s_w[s], o);
+      if (s < S && s_w[s] != 0.0f) o += x[k] * s_w[s];
     }
   }
   s_o[g][d] = o;
@@ -447,9 +508,12 @@ __global__ __launch_bounds__(256) void k_paged_join(JoinArgs a) {
 #pragma unroll
   for (int k = 1; k < NG; k++) o += s_o[k][d];
   const size_t row = (size_t)a.row0 + t;
-  float y = L > 0.0f ? o / L : L == 0.0f ? 0.0f : L;
-  if (a.gate) y *= gate_sigmoid((float)((const T *)a.gate)[row * a.gate_stride + (size_t)h * a.gate_head + d]);
-  ((T *)a.out)[(row * a.nh + h) * HD + d] = (T)y;
+  const float inv = L > 0.0f ? 1.0f / L : L;  // 0 stays, and a NaN
+  Pack<T, 4> y, gt;
+  if (a.gate) gt = *(const Pack<T, 4> *)((const T *)a.gate + row * a.gate_stride + (size_t)h * a.gate_head + 4 * d);
+#pragma unroll
+  for (int e = 0; e < 4; e++) y.v[e] = (T)(o[e] * inv * (a.gate ? gate_sigmoid((float)gt.v[e]) : 1.0f));
+  *(Pack<T, 4> *)((T *)a.out + (row * a.nh + h) * HD + 4 * d) = y;
 }
 
 // ---------------------------------------------------------------------------
@@ -974,11 +1038,11 @@ void launch_join(const JoinArgs &a, int hd, int rows, hipStream_t st) {
     b.pl += (size_t)r0 * a.nh;
     const dim3 grid(a.nh, n);
     if (hd == 64)
-      k_paged_join<T, 64><<<grid, 256, 0, st>>>(b);
+      k_paged_join<T, 64><<<grid, 512, 0, st>>>(b);
     else if (hd == 128)
-      k_paged_join<T, 128><<<grid, 256, 0, st>>>(b);
+      k_paged_join<T, 128><<<grid, 512, 0, st>>>(b);
     else
-      k_paged_join<T, 256><<<grid, 256, 0, st>>>(b);
+      k_paged_join<T, 256><<<grid, 512, 0, st>>>(b);
   }
 }
 
@@ -1102,21 +1166,44 @@ extern "C" int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *c, void *o
   a.scale = scale * kLog2e;
   a.map = page_map(c, table);
   const long long items = (long long)c->kv_heads * a.hgroups;
-  const int least = c->type == COLI_TYPE_F32 ? 64 : 128;  // one block a wave
+  const int least = c->type == COLI_TYPE_F32 ? DecodeShape<float, 64>::kLeast : DecodeShape<__bf16, 64>::kLeast;
+  const int per_cu = hd == 64    ? DecodeShape<__bf16, 64>::kPerCu
+                     : hd == 128 ? DecodeShape<__bf16, 128>::kPerCu
+                                 : DecodeShape<__bf16, 256>::kPerCu;
   for (int s0 = 0; s0 < sequences; s0 += kSeqs) {
     const int n = sequences - s0 < kSeqs ? sequences - s0 : kSeqs;
-    long long total = 0;
     int longest = 0;
+    long long total = 0;
     for (int r = 0; r < n; r++) {
       total += length[s0 + r];
       if (length[s0 + r] > longest) longest = length[s0 + r];
     }
-    // all splits of one length, two workgroups a compute unit in all
-    long long per = (total * items + 2 * cus_of(ctx) - 1) / (2 * cus_of(ctx));
-    if (per < (longest + kMaxSplits - 1) / kMaxSplits) per = (longest + kMaxSplits - 1) / kMaxSplits;
-    per = (per + least - 1) / least * least;
-    if (per < least) per = least;
-    a.per = per < INT_MAX / 2 ? (int)per : INT_MAX / 2 / least * least;
+    // All splits of one length: the least (in blocks of its waves) whose workgroups run
+    // at once.  Where that leaves much more to the longest split than an even share
+    // (many short sequences beside a long one), half that share, in more than one round.
+    const long long slots = (long long)per_cu * cus_of(ctx);
+    auto workgroups = [&](long long per) {
+      long long sum = 0;
+      for (int r = 0; r < n; r++) sum += length[s0 + r] <= per ? 1 : (length[s0 + r] + per - 1) / per;
+      return sum * items;
+    };
+    long long lo = ((longest + kMaxSplits - 1) / kMaxSplits + least - 1) / least, hi = ((long long)longest + least - 1) / least;
+    if (lo < 1) lo = 1;
+    if (hi < lo) hi = lo;
+    while (lo < hi) {  // the least in [lo, hi] that fits, or hi: one split a sequence
+      const long long mid = (lo + hi) / 2;
+      if (workgroups(mid * least) <= slots)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    const long long share = (total * items + slots - 1) / slots;
+    if (2 * lo * least > 3 * share) {
+      const long long half = (share / 2 + least - 1) / least, most = ((longest + kMaxSplits - 1) / kMaxSplits + least - 1) / least;
+      if (half < lo) lo = half > most ? half : most;
+      if (lo < 1) lo = 1;
+    }
+    a.per = (int)(lo * least < INT_MAX / 2 ? lo * least : INT_MAX / 2 / least * least);
     bool one = true;
     a.first[0] = 0;
     for (int r = 0; r < n; r++) {

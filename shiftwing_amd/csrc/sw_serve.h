@@ -56,6 +56,10 @@ __device__ __forceinline__ unsigned pack2(float lo, float hi) {
 // sigmoid of a gate: exp overflows to inf for far negative ones, which gives 0
 __device__ __forceinline__ float gate_sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
 
+// A barrier that waits for this wave's LDS accesses alone: __syncthreads would also
+// wait for loads in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // The last i with first[i] <= x among n + 1 ascending bounds in kernel arguments,
 // x < first[n]: every lane compares its own entries, so one load finds it.
 __device__ __forceinline__ int find_span(const int *first, int n, int x) {
