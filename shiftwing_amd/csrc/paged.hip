@@ -170,14 +170,15 @@ __device__ __forceinline__ v4f mfma_f32_16(float a, float b, v4f c) {
 // wave always has one of them in flight.
 // RUN16: pages hold whole runs of 16 positions, whose page the wave then looks up
 // once, by a scalar load, a block ahead; otherwise every lane looks up its own.
-template <class T, int HD>
+template <class T, int HD, bool RUN16>
 struct DecodeShape {
   static constexpr bool B16 = sizeof(T) == 2;
-  static constexpr int kPerCu = HD == 64 ? 3 : HD == 128 ? 2 : 1;  // workgroups of a compute unit, by their registers
+  // workgroups of a compute unit, by their registers (one lane's own look-ups take more)
+  static constexpr int kPerCu = HD == 64 ? (RUN16 ? 4 : 3) : HD == 128 ? (RUN16 ? 3 : 2) : 1;
   static constexpr int kLeast = 4 * (B16 ? 32 : 16);               // positions of a split: one block a wave
 };
 template <class T, int HD, bool RUN16>
-__global__ __launch_bounds__(256, (DecodeShape<T, HD>::kPerCu)) void k_paged_decode(DecodeArgs a) {
+__global__ __launch_bounds__(256, (DecodeShape<T, HD, RUN16>::kPerCu)) void k_paged_decode(DecodeArgs a) {
   constexpr bool B16 = sizeof(T) == 2;
   constexpr int NB = B16 ? 2 : 1, KB = 16 * NB;            // runs and positions of a block
   constexpr int NT = HD / 16;                              // dim tiles
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(256, (DecodeShape<T, HD>::kPerCu)) void k_paged_dec
   const int per_split = a.nkv * a.hgroups;
   const int slot = blockIdx.x / per_split, sub = blockIdx.x % per_split;
   const int kvh = sub / a.hgroups, hg = sub % a.hgroups;
-  const int r = find_span(a.first, a.rows, slot);
+  const int r = a.rows == 1 ? 0 : find_span(a.first, a.rows, slot);
   const int len = a.len[r];
   const int heads = min(16, a.G - 16 * hg), h0 = kvh * a.G + 16 * hg;
   const int key_first = (slot - a.first[r]) * a.per, key_end = min(len, key_first + a.per);
@@ -444,7 +445,9 @@ __global__ __launch_bounds__(256, (DecodeShape<T, HD>::kPerCu)) void k_paged_dec
 // Joins the splits of one (row, query head): the weights 2^(m - M) in LDS, while the
 // first outputs are on their way; a thread has four dims of every NG-th split, eight
 // loads in flight, and the groups meet in LDS in their order.
-// grid (query heads, rows), 512 threads, S <= kMaxSplits.
+// grid (query heads, rows); THREADS 512, or 128 where two rounds of theirs take all
+// splits and there are many (1,536 (row, head) pairs of 50 splits and less 11.2 -> 5.2
+// us); S <= kMaxSplits.
 constexpr int kMaxSplits = 256;
 struct JoinArgs {
   const float *po, *pm, *pl;
@@ -456,10 +459,11 @@ struct JoinArgs {
   long long row0;    // first row of out and gate
   int first[kSeqs + 1];  // flat: row r's records
 };
-template <class T, int HD>
-__global__ __launch_bounds__(512) void k_paged_join(JoinArgs a) {
-  constexpr int TH = HD / 4, NG = 512 / TH, B = 8;
-  __shared__ float s_w[kMaxSplits], s_red[16];
+constexpr int kJoinLoads = 8;  // of a thread in flight
+template <class T, int HD, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_paged_join(JoinArgs a) {
+  constexpr int TH = HD / 4, NG = THREADS / TH, B = kJoinLoads, NW = THREADS / 64;
+  __shared__ float s_w[THREADS < kMaxSplits ? THREADS : kMaxSplits], s_red[2 * NW];
   __shared__ v4f s_o[NG][TH];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, h = blockIdx.x, t = blockIdx.y;
   const int S = a.flat ? a.first[t + 1] - a.first[t] : a.S;
@@ -476,6 +480,9 @@ __global__ __launch_bounds__(512) void k_paged_join(JoinArgs a) {
     }
   };
   load(g);
+  const size_t row = (size_t)a.row0 + t;
+  Pack<T, 4> y, gt;
+  if (a.gate && g == 0) gt = *(const Pack<T, 4> *)((const T *)a.gate + row * a.gate_stride + (size_t)h * a.gate_head + 4 * d);
   const size_t rec = ((base + (size_t)(tid < S ? tid : 0) * step) * a.nh) + h;
   const float m = tid < S ? a.pm[rec] : -INFINITY, lv = tid < S ? a.pl[rec] : 0.0f;
   const float wm = wave_max_dpp(m);
@@ -483,15 +490,15 @@ __global__ __launch_bounds__(512) void k_paged_join(JoinArgs a) {
   __syncthreads();
   float M = s_red[0];
 #pragma unroll
-  for (int w = 1; w < 8; w++) M = fmaxf(M, s_red[w]);
+  for (int w = 1; w < NW; w++) M = fmaxf(M, s_red[w]);
   const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-  if (tid < kMaxSplits) s_w[tid] = w;
+  if (tid < S) s_w[tid] = w;
   const float ls = wave_sum_dpp(w == 0.0f ? 0.0f : lv * w);
-  if (lane == 0) s_red[8 + wave] = ls;
+  if (lane == 0) s_red[NW + wave] = ls;
   __syncthreads();
-  float L = s_red[8];
+  float L = s_red[NW];
 #pragma unroll
-  for (int k = 1; k < 8; k++) L += s_red[8 + k];
+  for (int k = 1; k < NW; k++) L += s_red[NW + k];
   v4f o = v4f{0.f, 0.f, 0.f, 0.f};
   for (int s0 = g; s0 < S; s0 += B * NG) {
     if (s0 != g) load(s0);
@@ -507,10 +514,7 @@ __global__ __launch_bounds__(512) void k_paged_join(JoinArgs a) {
   if (g) return;
 #pragma unroll
   for (int k = 1; k < NG; k++) o += s_o[k][d];
-  const size_t row = (size_t)a.row0 + t;
   const float inv = L > 0.0f ? 1.0f / L : L;  // 0 stays, and a NaN
-  Pack<T, 4> y, gt;
-  if (a.gate) gt = *(const Pack<T, 4> *)((const T *)a.gate + row * a.gate_stride + (size_t)h * a.gate_head + 4 * d);
 #pragma unroll
   for (int e = 0; e < 4; e++) y.v[e] = (T)(o[e] * inv * (a.gate ? gate_sigmoid((float)gt.v[e]) : 1.0f));
   *(Pack<T, 4> *)((T *)a.out + (row * a.nh + h) * HD + 4 * d) = y;
@@ -1027,8 +1031,16 @@ void launch_decode(const DecodeArgs &a, int hd, unsigned grid, hipStream_t st) {
     launch_decode<T, 256>(a, grid, st);
 }
 
+template <class T, int HD>
+void launch_join(const JoinArgs &a, int splits, dim3 grid, hipStream_t st) {
+  if (splits <= 2 * kJoinLoads * (128 / (HD / 4)) && (long long)grid.x * grid.y >= 1024)
+    k_paged_join<T, HD, 128><<<grid, 128, 0, st>>>(a);
+  else
+    k_paged_join<T, HD, 512><<<grid, 512, 0, st>>>(a);
+}
+// splits: of a row, at most
 template <class T>
-void launch_join(const JoinArgs &a, int hd, int rows, hipStream_t st) {
+void launch_join(const JoinArgs &a, int hd, int splits, int rows, hipStream_t st) {
   for (int r0 = 0; r0 < rows; r0 += 65535) {  // only rows of one split count (not flat) pass this limit
     JoinArgs b = a;
     const int n = rows - r0 < 65535 ? rows - r0 : 65535;
@@ -1038,15 +1050,14 @@ void launch_join(const JoinArgs &a, int hd, int rows, hipStream_t st) {
     b.pl += (size_t)r0 * a.nh;
     const dim3 grid(a.nh, n);
     if (hd == 64)
-      k_paged_join<T, 64><<<grid, 512, 0, st>>>(b);
+      launch_join<T, 64>(b, splits, grid, st);
     else if (hd == 128)
-      k_paged_join<T, 128><<<grid, 512, 0, st>>>(b);
+      launch_join<T, 128>(b, splits, grid, st);
     else
-      k_paged_join<T, 256><<<grid, 512, 0, st>>>(b);
+      launch_join<T, 256>(b, splits, grid, st);
   }
 }
 
-constexpr int kPromptRows = 128;
 template <class T, int HD, bool RUN>
 int launch_prompt(const char *name, const PromptArgs &a, dim3 grid, hipStream_t st) {
   typedef PromptShape<T, HD> Sh;
@@ -1062,7 +1073,8 @@ int launch_prompt(const char *name, const PromptArgs &a, dim3 grid, hipStream_t 
   return a.map.page_size % (Sh::kKeys / Sh::kWaves) == 0 ? launch_prompt<T, HD, true>(name, a, grid, st)
                                                          : launch_prompt<T, HD, false>(name, a, grid, st);
 }
-static_assert(PromptShape<float, 64>::kRows == kPromptRows && PromptShape<__bf16, 256>::kRows == kPromptRows, "rows of a tile");
+constexpr int kPromptRows = PromptShape<float, 64>::kRows;
+static_assert(PromptShape<__bf16, 256>::kRows == kPromptRows, "rows of a tile, the same for all");
 template <class T>
 int launch_prompt(const char *name, const PromptArgs &a, int hd, dim3 grid, hipStream_t st) {
   return hd == 64 ? launch_prompt<T, 64>(name, a, grid, st)
@@ -1166,10 +1178,11 @@ extern "C" int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *c, void *o
   a.scale = scale * kLog2e;
   a.map = page_map(c, table);
   const long long items = (long long)c->kv_heads * a.hgroups;
-  const int least = c->type == COLI_TYPE_F32 ? DecodeShape<float, 64>::kLeast : DecodeShape<__bf16, 64>::kLeast;
-  const int per_cu = hd == 64    ? DecodeShape<__bf16, 64>::kPerCu
-                     : hd == 128 ? DecodeShape<__bf16, 128>::kPerCu
-                                 : DecodeShape<__bf16, 256>::kPerCu;
+  const bool runs = c->page_size % 16 == 0;
+  const int least = c->type == COLI_TYPE_F32 ? DecodeShape<float, 64, true>::kLeast : DecodeShape<__bf16, 64, true>::kLeast;
+  const int per_cu = hd == 64    ? (runs ? DecodeShape<__bf16, 64, true>::kPerCu : DecodeShape<__bf16, 64, false>::kPerCu)
+                     : hd == 128 ? (runs ? DecodeShape<__bf16, 128, true>::kPerCu : DecodeShape<__bf16, 128, false>::kPerCu)
+                                 : DecodeShape<__bf16, 256, true>::kPerCu;
   for (int s0 = 0; s0 < sequences; s0 += kSeqs) {
     const int n = sequences - s0 < kSeqs ? sequences - s0 : kSeqs;
     int longest = 0;
@@ -1178,38 +1191,45 @@ extern "C" int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *c, void *o
       total += length[s0 + r];
       if (length[s0 + r] > longest) longest = length[s0 + r];
     }
-    // All splits of one length: the least (in blocks of its waves) whose workgroups run
-    // at once.  Where that leaves much more to the longest split than an even share
-    // (many short sequences beside a long one), half that share, in more than one round.
-    const long long slots = (long long)per_cu * cus_of(ctx);
-    auto workgroups = [&](long long per) {
-      long long sum = 0;
-      for (int r = 0; r < n; r++) sum += length[s0 + r] <= per ? 1 : (length[s0 + r] + per - 1) / per;
-      return sum * items;
-    };
-    long long lo = ((longest + kMaxSplits - 1) / kMaxSplits + least - 1) / least, hi = ((long long)longest + least - 1) / least;
+    // All splits of one length, in blocks of the four waves.  Where a compute unit holds
+    // one workgroup, the least length whose workgroups all run at once: 13 fp32
+    // sequences up to 6,000 positions 26 us, in two and three rounds 36 and 44; three
+    // bf16 ones up to 131,071 82 against 86 and 89.  Where it holds several (or one
+    // round leaves the longest split half as much again as an even share, beside many
+    // short sequences), a third of an even share, in rounds that level out: 48 fp16
+    // sequences up to 9,001 at head dim 128 160 us in one round, 145 / 143 / 143 at a
+    // half / third / quarter, at head dim 64 124 and 109 / 105 / 104.
+    const long long slots = (long long)per_cu * cus_of(ctx), share = (total * items + slots - 1) / slots;
+    const long long most = ((longest + kMaxSplits - 1) / kMaxSplits + least - 1) / least;  // kMaxSplits a sequence
+    long long lo = most, hi = ((long long)longest + least - 1) / least;
     if (lo < 1) lo = 1;
     if (hi < lo) hi = lo;
-    while (lo < hi) {  // the least in [lo, hi] that fits, or hi: one split a sequence
-      const long long mid = (lo + hi) / 2;
-      if (workgroups(mid * least) <= slots)
-        hi = mid;
-      else
-        lo = mid + 1;
+    if (per_cu == 1) {
+      auto workgroups = [&](long long per) {
+        long long sum = 0;
+        for (int r = 0; r < n; r++) sum += length[s0 + r] <= per ? 1 : (length[s0 + r] + per - 1) / per;
+        return sum * items;
+      };
+      while (lo < hi) {  // the least in [lo, hi] that fits, or hi: one split a sequence
+        const long long mid = (lo + hi) / 2;
+        if (workgroups(mid * least) <= slots)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
     }
-    const long long share = (total * items + slots - 1) / slots;
-    if (2 * lo * least > 3 * share) {
-      const long long half = (share / 2 + least - 1) / least, most = ((longest + kMaxSplits - 1) / kMaxSplits + least - 1) / least;
-      if (half < lo) lo = half > most ? half : most;
+    if (per_cu > 1 || 2 * lo * least > 3 * share) {
+      const long long third = (share / 3 + least - 1) / least;
+      lo = third > most ? third : most;
       if (lo < 1) lo = 1;
     }
     a.per = (int)(lo * least < INT_MAX / 2 ? lo * least : INT_MAX / 2 / least * least);
-    bool one = true;
+    int splits = 1;
     a.first[0] = 0;
     for (int r = 0; r < n; r++) {
       const int S = length[s0 + r] <= a.per ? 1 : (int)(((long long)length[s0 + r] + a.per - 1) / a.per);
       a.first[r + 1] = a.first[r] + S;
-      one = one && S == 1;
+      if (S > splits) splits = S;
     }
     memcpy(a.len, length + s0, n * sizeof(int));
     a.rows = n;
@@ -1218,7 +1238,7 @@ extern "C" int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *c, void *o
     a.out = (char *)out + (size_t)s0 * nh * hd * size;
     a.gate = gate ? (const char *)gate + (size_t)s0 * gate_stride * size : nullptr;
     a.po = a.pm = a.pl = nullptr;
-    if (!one && partials(ctx, name, a.first[n], nh, hd, &a.po, &a.pm, &a.pl)) return -1;
+    if (splits > 1 && partials(ctx, name, a.first[n], nh, hd, &a.po, &a.pm, &a.pl)) return -1;
     const unsigned grid = (unsigned)(a.first[n] * items);
     if (c->type == COLI_TYPE_F32)
       launch_decode<float>(a, hd, grid, ctx->stream);
@@ -1226,7 +1246,7 @@ extern "C" int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *c, void *o
       launch_decode<_Float16>(a, hd, grid, ctx->stream);
     else
       launch_decode<__bf16>(a, hd, grid, ctx->stream);
-    if (one) continue;
+    if (splits == 1) continue;
     JoinArgs j;
     memset(&j, 0, sizeof(j));
     j.po = a.po, j.pm = a.pm, j.pl = a.pl;
@@ -1238,11 +1258,11 @@ extern "C" int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *c, void *o
     j.flat = 1;
     memcpy(j.first, a.first, sizeof(a.first));
     if (c->type == COLI_TYPE_F32)
-      launch_join<float>(j, hd, n, ctx->stream);
+      launch_join<float>(j, hd, splits, n, ctx->stream);
     else if (c->type == COLI_TYPE_F16)
-      launch_join<_Float16>(j, hd, n, ctx->stream);
+      launch_join<_Float16>(j, hd, splits, n, ctx->stream);
     else
-      launch_join<__bf16>(j, hd, n, ctx->stream);
+      launch_join<__bf16>(j, hd, splits, n, ctx->stream);
   }
   return launch_status(name);
 }
@@ -1319,11 +1339,11 @@ extern "C" int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *c, void *o
     j.step = rows;
     j.row0 = start[s0];
     if (c->type == COLI_TYPE_F32)
-      launch_join<float>(j, hd, rows, ctx->stream);
+      launch_join<float>(j, hd, a.splits, rows, ctx->stream);
     else if (c->type == COLI_TYPE_F16)
-      launch_join<_Float16>(j, hd, rows, ctx->stream);
+      launch_join<_Float16>(j, hd, a.splits, rows, ctx->stream);
     else
-      launch_join<__bf16>(j, hd, rows, ctx->stream);
+      launch_join<__bf16>(j, hd, a.splits, rows, ctx->stream);
   }
   return launch_status(name);
 }
