@@ -213,7 +213,7 @@ __device__ __forceinline__ v4f mfma_f32_16(float a, float b, v4f c) {
 }
 __device__ __forceinline__ v4f mfma_b16(v4u a, v4u b, v4f c) { return Mat16<__bf16>::mul16(a, b, c); }
 constexpr int kPitchB = kKey * 2 + 16;  // bytes of a 16-bit row in LDS: 16 rows' pieces lie in distinct banks
-constexpr int kPitchF = kKey * 4 + 16;  // of an fp32 row
+constexpr int kPitchF = kKey / 2 * 4 + 16;  // of half an fp32 row
 
 // One workgroup a (chunk, key head).  The products of the chunk's keys with its keys
 // and queries, as raw rows (their lengths divide the results), serve every value head
@@ -259,54 +259,75 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
   const size_t gate_at = (size_t)(t0 + min(lane, n - 1)) * g.vh;
   const int h_first = hk * rep + (wave < rep ? wave : 0);
   float a_ = g.a[gate_at + h_first], b_ = g.b[gate_at + h_first], al_ = g.a_log[h_first], dt_ = g.dt_bias[h_first];
-  // raw rows, zero beyond the sequence's end and beyond key_dim
-  {
+  // Raw rows, zero beyond the sequence's end and beyond key_dim; fp32 ones in two halves,
+  // which lets a compute unit hold two workgroups.
+  constexpr int HALVES = sizeof(T) / 2, DP = kKey / HALVES;
+  v4f acc[5];  // tiles wave, wave + 4, ..
+#pragma unroll
+  for (int i = 0; i < 5; i++) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+  auto tile_of = [](int u, int &i, int &j) {  // row and column tile, of k k^T up to 9, then of q k^T
+    j = u < 10 ? u : u - 10;
+    i = 0;
+    while (j > i) j -= ++i;
+  };
+  float s2[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int half = 0; half < HALVES; half++) {
     const int t = threadIdx.x >> 2, p = threadIdx.x & 3;
 #pragma unroll
     for (int m = 0; m < 2; m++) {
       const T *src = m ? (const T *)g.q + (size_t)(t0 + t) * g.q_stride + (size_t)hk * g.dk
                        : (const T *)g.k + (size_t)(t0 + t) * g.k_stride + (size_t)hk * g.dk;
       char *row = lds + L::kWork + (m * kChunk + t) * kPitch;
-      float s2 = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kKey / 32; i++) {
-        const int c = p + 4 * i;
+      for (int i = 0; i < DP / 32; i++) {
+        const int c = p + 4 * i, d = half * DP + 8 * c;
         constexpr int V = sizeof(T) / 2;  // 16-byte pieces of eight elements
         v4u x[V];
 #pragma unroll
-        for (int u = 0; u < V; u++) x[u] = t < n && 8 * c < g.dk ? ((const v4u *)(src + 8 * c))[u] : v4u{0, 0, 0, 0};
+        for (int u = 0; u < V; u++) x[u] = t < n && d < g.dk ? ((const v4u *)(src + d))[u] : v4u{0, 0, 0, 0};
         float f[8];
         load8(f, (const T *)x);
 #pragma unroll
-        for (int e = 0; e < 8; e++) s2 = __builtin_fmaf(f[e], f[e], s2);
+        for (int e = 0; e < 8; e++) s2[m] = __builtin_fmaf(f[e], f[e], s2[m]);
 #pragma unroll
         for (int u = 0; u < V; u++) ((v4u *)(row + 8 * c * sizeof(T)))[u] = x[u];
       }
-      s2 += __shfl_xor(s2, 1);
-      s2 += __shfl_xor(s2, 2);
-      if (p == 0) (m ? s_qn : s_kn)[t] = 1.f / sqrtf(s2 + 1e-6f) * (m ? 1.f / sqrtf((float)g.dk) : 1.f);
-    }
-  }
-  __syncthreads();
-  for (int u = wave; u < 20; u += 4) {
-    int j = u < 10 ? u : u - 10, i = 0;
-    while (j > i) j -= ++i;
-    const char *ks = lds + L::kWork + (16 * j + n16) * kPitch;
-    const char *qt = lds + L::kWork + ((u < 10 ? 0 : kChunk) + 16 * i + n16) * kPitch;
-    v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
-    if constexpr (sizeof(T) == 2) {
-      for (int d = 0; d < g.dk; d += 32)
-        acc = Mat16<T>::mul16(*(const v4u *)(ks + 2 * d + 16 * kg), *(const v4u *)(qt + 2 * d + 16 * kg), acc);
-    } else {
-      for (int d = 0; d < g.dk; d += 16) {
-        const v4f x = *(const v4f *)(ks + 4 * d + 16 * kg), y = *(const v4f *)(qt + 4 * d + 16 * kg);
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc = mfma_f32_16(x[e], y[e], acc);
+      if (half == HALVES - 1) {
+        s2[m] += __shfl_xor(s2[m], 1);
+        s2[m] += __shfl_xor(s2[m], 2);
+        if (p == 0) (m ? s_qn : s_kn)[t] = 1.f / sqrtf(s2[m] + 1e-6f) * (m ? 1.f / sqrtf((float)g.dk) : 1.f);
       }
     }
+    __syncthreads();
+    const int dn = min(DP, g.dk - half * DP);
+#pragma unroll
+    for (int k = 0; k < 5; k++) {
+      int i, j;
+      tile_of(wave + 4 * k, i, j);
+      const char *ks = lds + L::kWork + (16 * j + n16) * kPitch;
+      const char *qt = lds + L::kWork + ((wave + 4 * k < 10 ? 0 : kChunk) + 16 * i + n16) * kPitch;
+      if constexpr (sizeof(T) == 2) {
+        for (int d = 0; d < dn; d += 32)
+          acc[k] = Mat16<T>::mul16(*(const v4u *)(ks + 2 * d + 16 * kg), *(const v4u *)(qt + 2 * d + 16 * kg), acc[k]);
+      } else {
+        for (int d = 0; d < dn; d += 16) {
+          const v4f x = *(const v4f *)(ks + 4 * d + 16 * kg), y = *(const v4f *)(qt + 4 * d + 16 * kg);
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[k] = mfma_f32_16(x[e], y[e], acc[k]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < 5; k++) {
+    const int u = wave + 4 * k;
+    int i, j;
+    tile_of(u, i, j);
     // row s = 16 j + 4 kg + e, column t = 16 i + n16
     const v4f kn = *(const v4f *)(s_kn + 16 * j + 4 * kg);
-    s_pair[u * 64 + lane] = acc * kn * (u < 10 ? s_kn : s_qn)[16 * i + n16];
+    s_pair[u * 64 + lane] = acc[k] * kn * (u < 10 ? s_kn : s_qn)[16 * i + n16];
   }
   __syncthreads();
 
