@@ -480,14 +480,16 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs g) {
 template <class T>
 struct ScanLds {
   static constexpr int NP = planes_of<T>();
-  static constexpr int kRows = kChunk * kPitchB;                // one plane of keys or queries
-  static constexpr int kPitchT = kChunk * 2 + 16;               // bytes of a column of 64 tokens
-  static constexpr int kTok = kSlice * kPitchT;                 // one plane of x or d
-  static constexpr int kState = kSlice * kPitchB;               // one plane of the state
+  static constexpr int kRows = kChunk * 256;   // one plane of keys or queries: [token][128]
+  static constexpr int kTok = kSlice * 128;    // one plane of x or d: [column][64 tokens]
+  static constexpr int kState = kSlice * 256;  // one plane of the state: [column][128]
   static constexpr int kK = 0, kQ = NP * kRows, kS = 2 * NP * kRows;
   static constexpr int kD = kS;                                 // d lies where the state was
   static constexpr int kX = kS + 3 * kState, kR = kX + 3 * kTok, kAll = kR + 3 * kTok;
 };
+// byte of a 16-byte chunk: rows of 16 chunks (keys, queries, state columns), of 8 (x, d)
+__device__ __forceinline__ int wide_at(int row, int chunk) { return row * 256 + ((chunk ^ chunk_xor<16>(row)) << 4); }
+__device__ __forceinline__ int tok_at(int row, int chunk) { return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4); }
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Wint-to-pointer-cast"
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -627,9 +629,9 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
     const int n = rows - c * kChunk;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      put_planes(lds + L::kK + lr * kPitchB + 16 * (lc + 8 * i), kraw[i]);
-      put_planes(lds + L::kQ + lr * kPitchB + 16 * (lc + 8 * i), qraw[i]);
-      put_split(lds + L::kS + (16 * ct + n16) * kPitchB + 2 * (32 * rt + 16 * i + 4 * kg), L::kState, S[i]);
+      put_planes(lds + L::kK + wide_at(lr, lc + 8 * i), kraw[i]);
+      put_planes(lds + L::kQ + wide_at(lr, lc + 8 * i), qraw[i]);
+      put_split(lds + L::kS + wide_at(16 * ct + n16, 4 * rt + 2 * i + (kg >> 1)) + 8 * (kg & 1), L::kState, S[i]);
     }
     const v4f v_ = v4f{(float)vv[0], (float)vv[1], (float)vv[2], (float)vv[3]};
     lds_barrier();
@@ -643,12 +645,12 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
       v4u kf[NP], qf[NP], sf[3];
 #pragma unroll
       for (int p = 0; p < NP; p++) {
-        kf[p] = *(const v4u *)(lds + L::kK + p * L::kRows + (16 * rt + n16) * kPitchB + 2 * d + 16 * kg);
-        qf[p] = *(const v4u *)(lds + L::kQ + p * L::kRows + (16 * rt + n16) * kPitchB + 2 * d + 16 * kg);
+        kf[p] = *(const v4u *)(lds + L::kK + p * L::kRows + wide_at(16 * rt + n16, d / 8 + kg));
+        qf[p] = *(const v4u *)(lds + L::kQ + p * L::kRows + wide_at(16 * rt + n16, d / 8 + kg));
       }
 #pragma unroll
       for (int p = 0; p < 3; p++)
-        sf[p] = *(const v4u *)(lds + L::kS + p * L::kState + (16 * ct + n16) * kPitchB + 2 * d + 16 * kg);
+        sf[p] = *(const v4u *)(lds + L::kS + p * L::kState + wide_at(16 * ct + n16, d / 8 + kg));
 #pragma unroll
       for (int p = 0; p < NP; p++)
 #pragma unroll
@@ -657,7 +659,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
           if (r + p < R::kParts) o = mfma_b16(qf[p], sf[r], o);
         }
     }
-    put_split(lds + L::kX + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, v_ - fx * ks);
+    put_split(lds + L::kX + tok_at(16 * ct + n16, 2 * rt + (kg >> 1)) + 8 * (kg & 1), L::kTok, v_ - fx * ks);
     o *= fq;
     lds_barrier();
     auto triangle = [&](v4f acc, const auto &tr, const char *b) {
@@ -667,7 +669,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
         if (2 * i > rt) break;
         v4u bf[parts];
 #pragma unroll
-        for (int p = 0; p < parts; p++) bf[p] = *(const v4u *)(b + p * L::kTok + (16 * ct + n16) * L::kPitchT + 64 * i + 16 * kg);
+        for (int p = 0; p < parts; p++) bf[p] = *(const v4u *)(b + p * L::kTok + tok_at(16 * ct + n16, 4 * i + kg));
 #pragma unroll
         for (int p = 0; p < parts; p++)
 #pragma unroll
@@ -677,8 +679,8 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
     };
     const v4f d = triangle(v4f{0.f, 0.f, 0.f, 0.f}, inv, lds + L::kX);
     if (c + 1 < c1) load_triangle(inv, R::kInv);
-    put_split(lds + L::kD + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, d, R::kParts);
-    put_split(lds + L::kR + (16 * ct + n16) * L::kPitchT + 2 * (16 * rt + 4 * kg), L::kTok, fr * d);
+    put_split(lds + L::kD + tok_at(16 * ct + n16, 2 * rt + (kg >> 1)) + 8 * (kg & 1), L::kTok, d, R::kParts);
+    put_split(lds + L::kR + tok_at(16 * ct + n16, 2 * rt + (kg >> 1)) + 8 * (kg & 1), L::kTok, fr * d);
     lds_barrier();
     o = triangle(o, pr, lds + L::kD);
     const float fe_ = fe;
@@ -702,14 +704,14 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
       v4u bf[3];
 #pragma unroll
       for (int p = 0; p < 3; p++)
-        bf[p] = *(const v4u *)(lds + L::kR + p * L::kTok + (16 * ct + n16) * L::kPitchT + 64 * i + 16 * kg);
+        bf[p] = *(const v4u *)(lds + L::kR + p * L::kTok + tok_at(16 * ct + n16, 4 * i + kg));
 #pragma unroll
       for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int p = 0; p < NP; p++) {
-          const char *kp = lds + L::kK + p * L::kRows + (32 * i + 8 * kg + (n16 >> 2)) * kPitchB +
-                           2 * (32 * rt + 16 * m + 4 * (n16 & 3));
-          const v2u lo = lds_transposed(kp), hi = lds_transposed(kp + 4 * kPitchB);
+          const char *kp = lds + L::kK + p * L::kRows + 8 * (n16 & 1);
+          const int row = 32 * i + 8 * kg + (n16 >> 2), chunk = 4 * rt + 2 * m + ((n16 & 3) >> 1);
+          const v2u lo = lds_transposed(kp + wide_at(row, chunk)), hi = lds_transposed(kp + wide_at(row + 4, chunk));
 #pragma unroll
           for (int r = 0; r + p < 3; r++) S[m] = mfma_b16(v4u{lo[0], lo[1], hi[0], hi[1]}, bf[r], S[m]);
         }

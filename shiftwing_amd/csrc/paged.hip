@@ -583,16 +583,6 @@ struct PromptShape {
 // (16 bits) or as single values (fp32).
 // LDS rows are stored with their 16-byte chunks exchanged by an XOR with the row
 // number, which spreads every access over all banks.
-// the XOR of a row of CPR chunks.  Bit by bit a sum of row bits, so that rows which
-// differ by a constant differ by a constant here too; chosen so that 16 rows of a
-// fragment of 32 or 16 columns, taken in the hardware's groups of 16 lanes, and the
-// rows that a transposing load takes together lie in distinct banks.
-template <int CPR>
-__host__ __device__ constexpr int chunk_xor(int r) {
-  return CPR == 8 ? ((r & 2) << 1) | ((r >> 1) & 2) | ((r >> 3) & 1)
-                  : ((r & 3) << 2) | (((r >> 1) ^ (r >> 2)) & 2) | ((r >> 3) & 1);
-}
-
 // Tile x of a launch, heavy ones first: tiles by their number within their sequence
 // (later ones see more), the sequences' last ones first.  Tile number l is preceded by
 // count(l + 1) tiles, count(l) = sum over sequences of max(0, tiles - l).

@@ -60,6 +60,17 @@ __device__ __forceinline__ float gate_sigmoid(float g) { return 1.0f / (1.0f + e
 // wait for loads in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Rows of 16-byte chunks in LDS without padding: chunk c of row r lies at c ^
+// chunk_xor(r).  For CPR chunks a row: bit by bit a sum of row bits, so that rows which
+// differ by a constant differ by a constant here too; chosen so that 16 rows of a
+// fragment of 32 or 16 columns, taken in the hardware's groups of 16 lanes, and the
+// rows that a transposing load takes together lie in distinct banks.
+template <int CPR>
+__host__ __device__ constexpr int chunk_xor(int r) {
+  return CPR == 8 ? ((r & 2) << 1) | ((r >> 1) & 2) | ((r >> 3) & 1)
+                  : ((r & 3) << 2) | (((r >> 1) ^ (r >> 2)) & 2) | ((r >> 3) & 1);
+}
+
 // The last i with first[i] <= x among n + 1 ascending bounds in kernel arguments,
 // x < first[n]: every lane compares its own entries, so one load finds it.
 __device__ __forceinline__ int find_span(const int *first, int n, int x) {
