@@ -491,9 +491,11 @@ __global__ __launch_bounds__(THREADS) void k_paged_join(JoinArgs a) {
   float M = s_red[0];
 #pragma unroll
   for (int w = 1; w < NW; w++) M = fmaxf(M, s_red[w]);
-  const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+  // a record without a visible position holds nothing and gets the weight -1: one of
+  // weight zero counts, for zero times a NaN is a NaN
+  const float w = m == -INFINITY ? -1.0f : __builtin_amdgcn_exp2f(m - M);
   if (tid < S) s_w[tid] = w;
-  const float ls = wave_sum_dpp(w == 0.0f ? 0.0f : lv * w);
+  const float ls = wave_sum_dpp(w < 0.0f ? 0.0f : lv * w);
   if (lane == 0) s_red[NW + wave] = ls;
   __syncthreads();
   float L = s_red[NW];
@@ -505,8 +507,7 @@ __global__ __launch_bounds__(THREADS) void k_paged_join(JoinArgs a) {
 #pragma unroll
     for (int k = 0; k < B; k++) {
       const int s = s0 + k * NG;
-      // a record without a visible position holds nothing
-      if (s < S && s_w[s] != 0.0f) o += x[k] * s_w[s];
+      if (s < S && !(s_w[s] < 0.0f)) o += x[k] * s_w[s];
     }
   }
   s_o[g][d] = o;

@@ -352,6 +352,33 @@ def test_prompt_more_sequences_than_a_launch(be):
             _check(got[r], want, tol, f"row {r} of sequence {s}")
 
 
+# ---- values that are not finite ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("call", ["decode", "prompt"])
+def test_a_nan_of_weight_zero(be, kind, call):
+    """A visible NaN (a key's, or a value's) among scores 400 below the largest: its weight is zero in fp32, in its
+    split and as its split's in the join, and zero times NaN is NaN."""
+    for what in ("key", "value"):
+        rng = np.random.default_rng(94)
+        lens, rows = [5000], 1 if call == "decode" else 3
+        c, table = _cache(be, kind, 2, 1, 64, 16, lens, rng)
+        K, V = _fill(c, table, lens, rng, kind)
+        q = np.zeros((rows, 2, 64), np.float32)
+        q[:, :, 0] = 8
+        pos = np.arange(5000)
+        K[table[0, pos // 16], pos % 16, :, 0] = np.where(pos < 2500, -25, 25)[:, None]
+        if what == "key":
+            K[table[0, 30 // 16], 30 % 16, 0, 5] = np.nan
+        else:
+            V[table[0, 30 // 16], 30 % 16, 0, 5] = np.nan
+        c.write(K, V)
+        got = c.decode(q, lens, 1.0) if call == "decode" else c.prompt(q, [0, rows], lens, 1.0)
+        hit = np.isnan(got)
+        assert np.all(hit if what == "key" else hit[:, :, 5] & (hit.sum(-1) == 1)), what
+
+
 # ---- together ---------------------------------------------------------------------------------------------
 
 
