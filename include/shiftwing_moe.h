@@ -574,8 +574,8 @@ enum { COLI_TYPE_F32 = 0, COLI_TYPE_F16 = 1, COLI_TYPE_BF16 = 2 };
  * written, and attention leaves them out.
  *
  * query_heads a multiple of kv_heads; head_dim 64, 128 or 256; pools 16-byte
- * aligned, page_stride a multiple of 8.  pages * page_size and
- * table_pages * page_size stay below 2^31. */
+ * aligned, page_stride a multiple of 8.  pages * page_size stays below 2^31,
+ * table_pages * page_size (the longest sequence) is at most 2^30. */
 typedef struct {
   int type; /* COLI_TYPE_*: queries, keys, values, gates, outputs, both pools */
   int query_heads, kv_heads, head_dim;
@@ -585,9 +585,9 @@ typedef struct {
 
 /* Packed sequences (host arrays): sequence s owns rows start[s] ..
  * start[s + 1] - 1 of the token tensors (start ascending from start[0] >= 0,
- * sequences + 1 entries), and they are the last of its length[s] cached
- * positions.  Rows of no sequence are neither read nor written.  A sequence
- * may have no row.
+ * sequences + 1 entries, fewer than 2^24 rows), and they are the last of its
+ * length[s] cached positions.  Rows of no sequence are neither read nor
+ * written.  A sequence may have no row.
  *
  * Appends the rows' keys and values to their pages, position rotation applied
  * on the way.  A head's vector is normalised first, x / rms(x) * (1 + norm)
@@ -598,7 +598,9 @@ typedef struct {
  * [rows][query_heads][head_dim]; q and q_out are both given or both NULL.
  * Row strides are elements from token to token, q_head_stride from query head
  * to query head (2 * head_dim where a gate lies behind each query), key and
- * value heads are contiguous; q_out must not overlap q. */
+ * value heads are contiguous; q_out must not overlap q.  Tensors are 16-byte
+ * aligned, strides non-negative multiples of 8; two rows whose tables give them
+ * the same cell race. */
 int coli_cuda_paged_append(ColiCuda *ctx, const ColiPaged *cache,
                            void *k_pool, void *v_pool, const int *table,
                            const int *start, const int *length, int sequences,
@@ -612,8 +614,11 @@ int coli_cuda_paged_append(ColiCuda *ctx, const ColiPaged *cache,
  * softmax(scale * q[s] . k_j) v_j over positions j < length[s] (host array) of
  * the cache, query head h on kv head h / (query_heads / kv_heads), times
  * sigmoid(gate) where gates are given (gate_stride elements from row to row,
- * gate_head_stride from head to head, both multiples of 4).  q and out are
- * contiguous and 16-byte aligned.  Sequences that see nothing get zeros. */
+ * gate_head_stride from head to head, both multiples of 4, the gates aligned to
+ * four elements).  q and out are contiguous and 16-byte aligned, scale is finite
+ * (negative or zero too).  Sequences that see nothing get zeros.  What lies in
+ * positions that a row does not see changes nothing, whatever it is; infinities
+ * and NaN in those it sees take their course. */
 int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *cache, void *out,
                            const void *q, const void *gate,
                            long long gate_stride, int gate_head_stride,
@@ -621,7 +626,8 @@ int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *cache, void *out,
                            const int *table, const int *length, int sequences,
                            float scale);
 /* The same for packed prompts (or chunks of them, or drafted tokens): row i of
- * the n rows of a sequence sees its positions up to length - n + i. */
+ * the n rows of a sequence sees its positions up to length - n + i.  rows *
+ * query_heads, in tiles of 128 for each sequence and kv head, at most 2^29. */
 int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *cache, void *out,
                            const void *q, const void *gate,
                            long long gate_stride, int gate_head_stride,
@@ -645,7 +651,13 @@ int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *cache, void *out,
  * itself or apart from it.  A call names a slot once.
  *
  * key_dim a multiple of 8 up to 128, value_dim of 32 up to 256; tensors 16-byte
- * aligned, strides multiples of 8. */
+ * aligned, strides non-negative multiples of 8.
+ *
+ * Inputs and states are finite, and so are the fp32 sums of squares of q and k.
+ * Otherwise the token's outputs and those after it are NaN where the rule reaches
+ * them, and in coli_cuda_delta_prompt, which takes 64 tokens at once, outputs of
+ * the same value head up to 63 tokens before it may be NaN too; other sequences
+ * and key heads keep theirs. */
 typedef struct {
   int type; /* COLI_TYPE_*: q, k, v, out */
   int key_heads, value_heads, key_dim, value_dim, slots;

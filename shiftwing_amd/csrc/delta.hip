@@ -831,7 +831,8 @@ extern "C" int coli_cuda_delta_prompt(ColiCuda *ctx, const ColiDelta *d, void *o
   if (sequences && !start) return fail_arg("%s: null start", name);
   if (sequences && start[0] < 0) return fail_arg("%s: start[0] is negative", name);
   for (int s = 0; s < sequences; s++)
-    if (start[s + 1] < start[s]) return fail_arg("%s: sequence %d has rows %d..%d", name, s, start[s], start[s + 1]);
+    if (start[s + 1] < start[s] || start[s + 1] > INT_MAX - kChunk)  // a chunk behind the last row is an int too
+      return fail_arg("%s: sequence %d has rows %d..%d", name, s, start[s], start[s + 1]);
   if (!ctx) return fail_arg("%s: null context", name);
   OnDevice on(ctx);
   DeltaArgs g;

@@ -956,8 +956,10 @@ bool pools_ok(const char *name, const ColiPaged *c, const void *k_pool, const vo
     return fail_arg("%s: query_heads %d (1..65535) must be a multiple of kv_heads %d", name, c->query_heads, c->kv_heads),
            false;
   if (c->page_size <= 0 || c->pages <= 0 || c->table_pages <= 0 || (long long)c->pages * c->page_size > INT_MAX ||
-      (long long)c->table_pages * c->page_size > INT_MAX)
-    return fail_arg("%s: page_size, pages and table_pages must be positive, their products below 2^31", name), false;
+      (long long)c->table_pages * c->page_size > 1 << 30)  // a tile behind the last position is an int too
+    return fail_arg("%s: page_size, pages and table_pages must be positive, pages * page_size below 2^31, "
+                    "table_pages * page_size at most 2^30", name),
+           false;
   const long long page = (long long)c->page_size * c->kv_heads * c->head_dim;
   if (c->page_stride < page || c->page_stride % 8 || c->page_stride > LLONG_MAX / 8 / c->pages)
     return fail_arg("%s: page_stride %lld must be a multiple of 8 and at least one page's %lld elements", name,
@@ -969,9 +971,13 @@ bool pools_ok(const char *name, const ColiPaged *c, const void *k_pool, const vo
   return true;
 }
 
+constexpr int kMostRows = (1 << 24) - 1;
 bool rows_ok(const char *name, const ColiPaged *c, const int *start, const int *length, int sequences) {
   if (sequences < 0 || (sequences && !length)) return fail_arg("%s: null lengths or negative sequence count", name), false;
   if (start && sequences && start[0] < 0) return fail_arg("%s: start[0] is negative", name), false;
+  // a launch takes fewer than 2^32 threads
+  if (start && sequences && (long long)start[sequences] - start[0] > kMostRows)
+    return fail_arg("%s: %d rows in a call, more than 2^24 - 1", name, start[sequences] - start[0]), false;
   for (int s = 0; s < sequences; s++) {
     if (length[s] < 0 || length[s] > (long long)c->table_pages * c->page_size)
       return fail_arg("%s: length[%d] = %d is outside 0..%lld", name, s, length[s], (long long)c->table_pages * c->page_size),
@@ -1032,21 +1038,13 @@ void launch_join(const JoinArgs &a, int splits, dim3 grid, hipStream_t st) {
 // splits: of a row, at most
 template <class T>
 void launch_join(const JoinArgs &a, int hd, int splits, int rows, hipStream_t st) {
-  for (int r0 = 0; r0 < rows; r0 += 65535) {  // only rows of one split count (not flat) pass this limit
-    JoinArgs b = a;
-    const int n = rows - r0 < 65535 ? rows - r0 : 65535;
-    b.row0 += r0;
-    b.po += (size_t)r0 * a.nh * hd;
-    b.pm += (size_t)r0 * a.nh;
-    b.pl += (size_t)r0 * a.nh;
-    const dim3 grid(a.nh, n);
-    if (hd == 64)
-      launch_join<T, 64>(b, splits, grid, st);
-    else if (hd == 128)
-      launch_join<T, 128>(b, splits, grid, st);
-    else
-      launch_join<T, 256>(b, splits, grid, st);
-  }
+  const dim3 grid(a.nh, rows);  // a prompt in splits has fewer tiles of 128 rows than there are compute units
+  if (hd == 64)
+    launch_join<T, 64>(a, splits, grid, st);
+  else if (hd == 128)
+    launch_join<T, 128>(a, splits, grid, st);
+  else
+    launch_join<T, 256>(a, splits, grid, st);
 }
 
 template <class T, int HD, bool RUN>
@@ -1268,9 +1266,11 @@ extern "C" int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *c, void *o
   if (!out || !q || !aligned16(out) || !aligned16(q)) return fail_arg("%s: q and out must be 16-byte aligned", name);
   if (!isfinite(scale)) return fail_arg("%s: scale is not finite", name);
   const int nh = c->query_heads, hd = c->head_dim, G = nh / c->kv_heads, R = kPromptRows;
-  for (int s = 0; s < sequences; s++)
-    if ((long long)(start[s + 1] - start[s]) * G > INT_MAX - R)
-      return fail_arg("%s: sequence %d has %d rows of %d heads a kv head: more than 2^31", name, s, start[s + 1] - start[s], G);
+  // (token, head) rows of a call, which also bounds a launch's threads: 256 a tile of 128
+  // rows, or 512 at head_dim 256
+  long long all = 0;
+  for (int s = 0; s < sequences; s++) all += ((long long)(start[s + 1] - start[s]) * G + R - 1) / R * R * c->kv_heads;
+  if (all > 1 << 29) return fail_arg("%s: %lld (row, query head) pairs in tiles of %d, more than 2^29", name, all, R);
   if (!ctx) return fail_arg("%s: null context", name);
   OnDevice on(ctx);
   PromptArgs a;
@@ -1296,7 +1296,6 @@ extern "C" int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *c, void *o
     for (int s = 0; s < n; s++) {
       const int m = start[s0 + s + 1] - start[s0 + s];
       tiles += ((long long)m * G + R - 1) / R;
-      if (tiles * c->kv_heads > INT_MAX) return fail_arg("%s: too many rows", name);
       a.tile0[s + 1] = (int)tiles;
       if (m && length[s0 + s] > longest) longest = length[s0 + s];
     }

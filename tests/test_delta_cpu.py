@@ -68,3 +68,5 @@ def test_prompt_rows():
     _refused(_prompt(start=None), "null start")
     _refused(_prompt(start=[-1, 5, 5]), "negative")
     _refused(_prompt(start=[0, 5, 4]), "sequence 1")
+    _refused(_prompt(start=[0, 5, (1 << 31) - 64]), "sequence 1")
+    _refused(_prompt(start=[0, 5, (1 << 31) - 65]), "null context")

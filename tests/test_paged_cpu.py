@@ -127,3 +127,18 @@ def test_append_operands():
     # what is not used is not looked at
     _refused(_append(rd=0, theta=0.0), "null context")
     _refused(_append(q_norm=None, k_norm=None, eps=-1.0), "null context")
+
+
+def test_largest_sizes():
+    """Sizes whose indexes or launches would not fit: refused before anything runs."""
+    many = _cache(table_pages=(1 << 26) + 1)
+    for call in (_append, _decode, _prompt):
+        _refused(call(many), "2^30")
+    most = dict(table_pages=1 << 26)
+    _refused(_append(_cache(**most), start=[0, 1 << 23, 1 << 24], length=[1 << 30, 1 << 23]), "2^24 - 1")
+    _refused(_prompt(_cache(**most), start=[0, 1 << 23, 1 << 24], length=[1 << 30, 1 << 23]), "2^24 - 1")
+    _refused(_append(_cache(**most), start=[5, 1 << 23, (1 << 24) + 4], length=[1 << 30, 1 << 30]), "null context")
+    _refused(_prompt(_cache(**most), start=[5, 1 << 23, (1 << 24) + 4], length=[1 << 30, 1 << 30]), "null context")
+    heads = dict(query_heads=1024, kv_heads=2, **most)  # 512 a kv head: 2^20 tokens of 1,024 heads
+    _refused(_prompt(_cache(**heads), start=[0, 1 << 19, (1 << 19) + 1], length=[1 << 20, 1]), "2^29")
+    _refused(_prompt(_cache(**heads), start=[0, 1 << 18, 1 << 19], length=[1 << 20, 1 << 20]), "null context")
