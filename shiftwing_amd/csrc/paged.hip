@@ -905,6 +905,65 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, 
     }
   }
   l_run = over_groups(l_run, [](float x, float y) { return x + y; });
+
+  // A position of a tile that a row does not see has the probability zero, and zero times
+  // an infinite or NaN value is NaN.  Rows of the wave that are not finite are formed anew
+  // from what they see, one by one, if one of the positions unseen by the first row
+  // holds such a value: nothing any ordinary prompt pays for.
+  float zero = 0.0f;
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int i = 0; i < NA; i++) zero += o[d][i] * 0.0f;
+  unsigned long long odd = __ballot(live && zero != 0.0f);
+  if (odd) {
+    constexpr int E = HD / 64;  // dims of a lane
+    typedef Pack<T, E> P;
+    const int behind = min(key_end, key_first + ((wave_any - key_first) / KT + 1) * KT);
+    bool hidden = false;
+    for (int p = max(key_first, wave_all + 1); p < behind; p++) {
+      const long long at = cell(a.map, tab, p);
+      if (at < 0) continue;
+      const P x = *(const P *)(vc + at + E * lane);
+#pragma unroll
+      for (int e = 0; e < E; e++) hidden |= (float)x.v[e] * 0.0f != 0.0f;
+    }
+    if (!__any(hidden)) odd = 0;
+    for (int r = 0; r < C; r++) {
+      if (!(odd >> r & (NG == 4 ? 0x1000100010001ull : 0x100000001ull))) continue;
+      const int end = min(key_end, base + __shfl(tok, r) + 1);
+      const float m = __shfl(m_ref == -INFINITY ? 0.0f : m_ref, r), sign = a.q_sign ? -a.scale : a.scale;
+      const T *qp = (const T *)a.q + ((size_t)(a.start[s] + __shfl(tok, r)) * a.nh + __shfl(head, r)) * HD;
+      float x[E] = {};
+      for (int p0 = key_first; p0 < end; p0 += 64) {  // a lane a position, then all lanes a value
+        const long long at = p0 + lane < end ? cell(a.map, tab, p0 + lane) : -1;
+        const T *kp = kc + (at < 0 ? 0 : at);
+        float w = 0.0f;
+        for (int d = 0; d < HD; d += 4) {
+          const Pack<T, 4> kv = *(const Pack<T, 4> *)(kp + d), qv = *(const Pack<T, 4> *)(qp + d);
+#pragma unroll
+          for (int e = 0; e < 4; e++) w = __builtin_fmaf((float)kv.v[e], (float)qv.v[e], w);
+        }
+        w = __builtin_amdgcn_exp2f(__builtin_fmaf(w, sign, -m));
+        for (int j = 0; j < min(64, end - p0); j++) {
+          const long long from = __shfl(at, j);
+          if (from < 0) continue;
+          const float wj = __shfl(w, j);
+          const P v = *(const P *)(vc + from + E * lane);
+#pragma unroll
+          for (int e = 0; e < E; e++) x[e] = __builtin_fmaf(wj, (float)v.v[e], x[e]);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < NA; i++) {
+          const int dim = C * d + 4 * NG * (i / 4) + 4 * g + i % 4;
+          const float y = __shfl(x[i % E], dim / E);
+          if (c == r) o[d][i] = y;
+        }
+    }
+  }
   if (!live) return;
   if (a.po) {
     const size_t rec = ((size_t)split * a.rows + (a.start[s] - a.start[0] + tok)) * a.nh + head;

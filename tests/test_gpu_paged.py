@@ -379,6 +379,40 @@ def test_a_nan_of_weight_zero(be, kind, call):
         assert np.all(hit if what == "key" else hit[:, :, 5] & (hit.sum(-1) == 1)), what
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nh,nkv,hd,ps,start,lens,at", [
+    (2, 2, 64, 16, [0, 70], [70], [69]),                    # the last row's own
+    (4, 2, 128, 16, [0, 150, 180], [150, 400], [77, 395]),  # within a prompt, and behind a cached prefix
+    (16, 2, 256, 16, [0, 45], [45], [20]),
+    (6, 2, 256, 6, [0, 90], [130], [100]),                  # pages that end inside tiles
+    (8, 1, 64, 64, [0, 7], [3000], [2996]),                 # splits
+    (3, 1, 128, 16, [0, 40], [50], [3]),                    # seen by every row
+])
+def test_prompt_values_that_are_not_seen(be, kind, nh, nkv, hd, ps, start, lens, at):
+    """A NaN among the values of one position, an infinity beside it: rows before it are as they would be, the others
+    have it in that dim alone."""
+    rng = np.random.default_rng(95)
+    c, table = _cache(be, kind, nh, nkv, hd, ps, lens, rng)
+    K, V = _fill(c, table, lens, rng, kind)
+    clean = V.copy()
+    for s, p in enumerate(at):
+        V[table[s, p // ps], p % ps, :, 3], V[table[s, p // ps], p % ps, :, hd - 2] = np.nan, -np.inf
+    c.write(K, V)
+    q = _round(rng.standard_normal((start[-1], nh, hd)), kind)
+    for scale in (hd ** -0.5, -0.03):
+        got = c.prompt(q, start, lens, scale)
+        for s, n in enumerate(lens):
+            for r in range(start[s], start[s + 1]):
+                sees = n - (start[s + 1] - r) + 1
+                want, tol = _want(q[r], K, clean, table, s, sees, float(np.float32(scale)), None, kind)
+                if s < len(at) and sees > at[s]:
+                    assert np.all(np.isnan(got[r, :, 3])) and np.all(got[r, :, hd - 2] == -np.inf)
+                    rest = [d for d in range(hd) if d not in (3, hd - 2)]
+                else:
+                    rest = list(range(hd))
+                _check(got[r][:, rest], want[:, rest], tol[:, rest], f"row {r} of sequence {s}, scale {scale}")
+
+
 # ---- together ---------------------------------------------------------------------------------------------
 
 
