@@ -210,3 +210,88 @@ def test_same_state_as_the_layer(be, oracle):
     r.size = np.sqrt((r.S ** 2).sum(2, keepdims=True))
     r.run_prompt(*r.rows(66), [0, 66], [1])
     assert np.array_equal(dev.read_state()[1], r.dev.read())
+
+
+class Raw:
+    """The C calls on q, k and v of their own."""
+
+    def __init__(self, be, r, strides):
+        import ctypes as C
+
+        from shiftwing_amd.abi import ColiDelta
+        from shiftwing_amd.paged import KINDS
+        self.C, self.be, self.r = C, be, r
+        self.d = ColiDelta(KINDS[r.kind], r.kh, r.vh, r.dk, r.dv, r.dev.slots, *strides)
+
+    def call(self, name, out, q, k, v, a, b, *rest):
+        ints = [(self.C.c_int * len(x))(*x) if isinstance(x, list) else x for x in rest]
+        dev = self.r.dev
+        self.be.check(getattr(self.be.lib, "coli_cuda_delta_" + name)(
+            self.be.ctx, self.C.byref(self.d), out.p, q.p, k.p, v.p, a.p, b.p, dev.a_log.p, dev.dt_bias.p, dev.state.p,
+            dev.state.p, *ints), name)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_tensors_apart(be, kind):
+    """q, k and v in arrays and strides of their own, an output that is not clear, rows of no sequence, which may hold
+    anything."""
+    from shiftwing_amd.paged import from_kind, to_kind, word
+    r = Rule(be, kind, 2, 6, 72, 96, 5, 31)
+    T, kd, vd = 150, 2 * 72, 6 * 96
+    mix, a, b = r.rows(T)
+    start, slot = [4, 70, 147], [3, 1]
+    mix[:4], mix[147:], a[:4], b[147:] = np.nan, np.inf, np.nan, np.nan
+    parts = [mix[:, :kd], mix[:, kd:2 * kd], mix[:, 2 * kd:]]
+    wide = [kd + 8, kd, vd + 40]
+    dev = [be.upload(to_kind(np.concatenate([x, np.full((T, w - x.shape[1]), np.nan, np.float32)], 1), kind))
+           for x, w in zip(parts, wide)]
+    da, db = be.upload(a), be.upload(b)
+    raw = Raw(be, r, wide)
+    out = be.upload(to_kind(np.full((T, 6, 96), 7.0), kind))
+    raw.call("prompt", out, *dev, da, db, start, slot, 2)
+    got = from_kind(be.download(out, (T, 6, 96), word(kind)), kind)
+    assert np.all(got[:4] == 7.0) and np.all(got[147:] == 7.0)
+    mix[:4], mix[147:], a[:4], b[147:] = 0, 0, 0, 0
+    want = r.prompt(mix, a, b, start, slot)
+    for s in range(2):
+        rows = slice(start[s], start[s + 1])
+        r.check_out(got[rows], want[rows], np.full(start[s + 1] - start[s], slot[s]), f"sequence {s}")
+    r.check_state()
+    mix, a, b = r.rows(2)
+    dev = [be.upload(to_kind(np.concatenate([x, np.full((2, w - x.shape[1]), np.nan, np.float32)], 1), kind))
+           for x, w in zip((mix[:, :kd], mix[:, kd:2 * kd], mix[:, 2 * kd:]), wide)]
+    da, db = be.upload(a), be.upload(b)
+    raw.call("step", out, *dev, da, db, [4, 3], 2)
+    want = r.token(mix, a, b, np.array([4, 3]))
+    r.chunks[[4, 3]] += 1
+    got = from_kind(be.download(out, (T, 6, 96), word(kind)), kind)
+    r.check_out(got[:2], want, np.array([4, 3]), "step")
+    r.check_state()
+
+
+def test_what_is_not_finite_stays_with_its_sequence(be):
+    """A NaN in one sequence: another, and the slots no call names, are as without it, to the bit; from the NaN on its
+    own outputs and its state are NaN."""
+    got = []
+    for bad in (False, True):
+        r = Rule(be, "bf16", 2, 4, 128, 64, 3, 32)
+        mix, a, b = r.rows(300)
+        if bad:
+            mix[100, :2 * 2 * 128] = np.nan  # q and k
+        got.append((r.dev.prompt(mix, a, b, [0, 170, 300], [2, 0]), r.dev.read()))
+    (clean, state), (out, after) = got
+    assert np.array_equal(out[170:], clean[170:]) and np.array_equal(out[:64], clean[:64])
+    assert np.array_equal(after[[0, 1]], state[[0, 1]])
+    assert np.all(np.isnan(out[100:170])) and np.all(np.isnan(after[2]))
+
+
+def test_the_same_bits_again(be):
+    r = Rule(be, "bf16", 2, 8, 128, 128, 4, 33)
+    mix, a, b = r.rows(700)
+    before, seen = r.dev.read(), []
+    for _ in range(3):
+        r.dev.write(before)
+        out = r.dev.prompt(mix, a, b, [0, 333, 334, 700], [1, 3, 0])
+        seen.append((out, r.dev.step(mix[:4], a[:4], b[:4], [0, 1, 2, 3]), r.dev.read()))
+    for other in seen[1:]:
+        assert all(np.array_equal(x, y) for x, y in zip(seen[0], other))

@@ -446,3 +446,113 @@ def test_prompts_then_tokens(be, kind):
                 want, tol = _want(rq[r], K, V, table, s, have[s] - (start[s + 1] - r) + 1, scale, gate[r], kind)
                 _check(got[r], want, tol, f"row {r}")
     assert have == final
+
+
+# ---- calls that the wrapper does not make --------------------------------------------------------------------
+
+
+class Raw:
+    """The C calls on device buffers of one's own, on any context."""
+
+    def __init__(self, be, kind, nh, nkv, hd, ps, pages, width, stride=0):
+        import ctypes as C
+
+        from shiftwing_amd.abi import ColiPaged
+        from shiftwing_amd.paged import KINDS
+        self.C, self.be, self.kind, self.nh, self.hd = C, be, kind, nh, hd
+        self.c = ColiPaged(KINDS[kind], nh, nkv, hd, ps, pages, width, stride or ps * nkv * hd)
+
+    def ints(self, a):
+        return (self.C.c_int * len(a))(*a)
+
+    def call(self, name, *args):
+        self.be.check(getattr(self.be.lib, name)(self.be.ctx, self.C.byref(self.c), *args), name)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_gates_behind_the_queries(be, kind):
+    """Gates as the projection leaves them, behind each head's query, in rows wider than that; an output that is
+    not clear, whose rows of no sequence stay; scales of zero and below."""
+    from shiftwing_amd.paged import from_kind, to_kind, word
+    rng = np.random.default_rng(101)
+    nh, nkv, hd, ps, start, lens = 6, 2, 128, 16, [1, 40, 43], [39, 900]
+    c, table = _cache(be, kind, nh, nkv, hd, ps, lens, rng)
+    K, V = _fill(c, table, lens, rng, kind)
+    r = Raw(be, kind, nh, nkv, hd, ps, c.shape[0], table.shape[1])
+    rows, wide, size = 45, nh * 2 * hd + 20, np.dtype(word(kind)).itemsize
+    mix = _round(rng.standard_normal((rows, wide)) * 2, kind)
+    gate = mix[:, :nh * 2 * hd].reshape(rows, nh, 2, hd)[:, :, 1]
+    q = _round(rng.standard_normal((rows, nh, hd)), kind)
+    dmix, dq = be.upload(to_kind(mix, kind)), be.upload(to_kind(q, kind))
+    for scale in (0.0, -0.05):
+        for name, args, n in (("prompt", (r.ints(start), r.ints(lens), 2), rows), ("decode", (r.ints(lens), 2), 2)):
+            out = be.upload(to_kind(np.full((rows, nh, hd), 7.0), kind))
+            r.call("coli_cuda_paged_" + name, out.p, dq.p, r.C.c_void_p(dmix.ptr + hd * size), wide, 2 * hd, c.k_pool.p,
+                   c.v_pool.p, c.table.p, *args, scale)
+            got = from_kind(be.download(out, (rows, nh, hd), word(kind)), kind)
+            seen = np.zeros(rows, bool)
+            for s, length in enumerate(lens):
+                mine = range(start[s], start[s + 1]) if name == "prompt" else [s]
+                for i, row in enumerate(mine):
+                    seen[row] = True
+                    sees = length - len(mine) + i + 1
+                    want, tol = _want(q[row], K, V, table, s, sees, float(np.float32(scale)), gate[row], kind)
+                    _check(got[row], want, tol, f"{name} row {row} scale {scale}")
+            assert np.all(got[~seen] == 7.0)
+
+
+def test_a_pool_beyond_32_bits(be):
+    """Pages 2^30 elements apart: the last one begins 2^32 elements (8 GiB) behind the first."""
+    from shiftwing_amd.paged import from_kind, to_kind
+    rng = np.random.default_rng(102)
+    nh, nkv, hd, ps, T = 4, 2, 64, 16, 40
+    row, far = nkv * hd, 1 << 30
+    r = Raw(be, "bf16", nh, nkv, hd, ps, 5, 3, far)
+    pool = be.alloc((4 * far + 2 * ps * row) * 2)
+    v_pool = r.C.c_void_p(pool.ptr + ps * row * 2)  # behind each page's keys
+    table = be.upload(np.array([[4, 0, 3]], np.int32))
+    k, v = (_round(rng.standard_normal((T, nkv, hd)), "bf16") for _ in range(2))
+    q = _round(rng.standard_normal((T, nh, hd)), "bf16")
+    dk, dv, dq = (be.upload(to_kind(x, "bf16")) for x in (k, v, q))
+    r.call("coli_cuda_paged_append", pool.p, v_pool, table.p, r.ints([0, T]), r.ints([T]), 1, None, None, 0, 0, dk.p, row, dv.p,
+           row, None, None, 0.0, 0, 0.0)
+    out = be.alloc(T * nh * hd * 2)
+    r.call("coli_cuda_paged_prompt", out.p, dq.p, None, 0, 0, pool.p, v_pool, table.p, r.ints([0, T]), r.ints([T]), 1, 0.125)
+    prompt = from_kind(be.download(out, (T, nh, hd), np.uint16), "bf16")
+    r.call("coli_cuda_paged_decode", out.p, dq.p, None, 0, 0, pool.p, v_pool, table.p, r.ints([T]), 1, 0.125)
+    token = from_kind(be.download(out, (1, nh, hd), np.uint16), "bf16")
+    flat = np.zeros((3, ps, nkv, hd), np.float32), np.zeros((3, ps, nkv, hd), np.float32)
+    for x, y in zip(flat, (k, v)):
+        x.reshape(-1, nkv, hd)[:T] = y
+    plain = np.arange(3)[None]
+    for i in range(T):
+        want, tol = _want(q[i], *flat, plain, 0, i + 1, 0.125, None, "bf16")
+        _check(prompt[i], want, tol, f"row {i}")
+    want, tol = _want(q[0], *flat, plain, 0, T, 0.125, None, "bf16")
+    _check(token[0], want, tol, "the token")
+
+
+def test_two_contexts_and_the_same_call_again(be):
+    """Calls queued on two contexts in turn, with different sizes of workspace, repeated: the same bits each time."""
+    from shiftwing_amd import Backend
+    rng = np.random.default_rng(103)
+    other = Backend(0)
+    cases = []
+    for b, lens in ((be, [3000, 17]), (other, [901, 64, 1, 2500])):
+        c, table = _cache(b, "bf16", 8, 2, 128, 16, lens, rng)
+        _fill(c, table, lens, rng, "bf16")
+        r = Raw(b, "bf16", 8, 2, 128, 16, c.shape[0], table.shape[1])
+        q = b.upload(rng.integers(0, 2, (len(lens), 8, 128)).astype(np.uint16) + 0x3F80)
+        outs = [b.alloc(len(lens) * 8 * 128 * 2) for _ in range(6)]
+        cases.append((b, c, r, q, outs, lens))
+    for turn in range(6):
+        for b, c, r, q, outs, lens in cases:
+            n = len(lens)
+            extra = (r.ints(list(range(n + 1))),) if turn % 2 else ()
+            r.call("coli_cuda_paged_" + ("prompt" if turn % 2 else "decode"), outs[turn].p, q.p, None, 0, 0, c.k_pool.p,
+                   c.v_pool.p, c.table.p, *extra, r.ints(lens), n, 0.09)
+    for b, c, r, q, outs, lens in cases:
+        got = [b.download(o, (len(lens) * 8 * 128,), np.uint16) for o in outs]
+        for turn in range(2, 6):
+            assert np.array_equal(got[turn], got[turn % 2]), f"turn {turn}"
+        assert np.any(got[0] != 0)
