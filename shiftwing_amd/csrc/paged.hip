@@ -64,10 +64,13 @@ struct alignas(sizeof(T) * E) Pack {
 };
 
 // One workgroup a (token, run of heads), one wave a head: E = HD / 64 elements a
-// lane.  HBM-bound (each value read and written once).  The angle is formed once a
+// lane.  HBM-bound (each value read and written once): 6,379 fp32 tokens of 16 + 2
+// heads of 256 (261 MB) 54 us, 4.8 TB/s, where a large copy reaches 5.1; one bf16
+// token 4.2 us, the launch and its chain of loads.  The angle is formed once a
 // workgroup: turns = position * freq in 64 bits, the whole turns dropped, the rest
 // to fp32 (2^-25 turns), so far positions keep theirs.  The rotation's partners meet
-// in LDS, where any even rotary_dim finds them.
+// in LDS, where any even rotary_dim finds them.  The result is rounded to the cache's
+// type once; sums of squares are fp32.
 template <class T, int HD>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   constexpr int E = HD / 64;
@@ -167,7 +170,12 @@ __device__ __forceinline__ v4f mfma_f32_16(float a, float b, v4f c) {
 // row n of dim tile d stands for dim W n + d (tiles of one load).
 // Nothing goes through LDS until the waves' merge.  HBM-bound: a block's keys are
 // loaded as soon as the last ones' registers are free, its values likewise, so that a
-// wave always has one of them in flight.
+// wave always has one of them in flight.  Every key and value is fetched once (466 MB
+// counted for 466 MB): 227,641 bf16 positions of 2 kv heads x 256 83 us, 5.6 TB/s; 48
+// fp16 sequences up to 9,001 at 8 x 128 142 us, 5.1 TB/s; 13 fp32 ones up to 6,000 27
+// us, 5.2 TB/s; one of 4,097 positions 8.5 us, of which 1.6 would be the bytes' own.
+// A probability is rounded to the cache's 16 bits for the second product, half a step
+// of what the values themselves are rounded to; fp32 caches take fp32 products.
 // RUN16: pages hold whole runs of 16 positions, whose page the wave then looks up
 // once, by a scalar load, a block ahead; otherwise every lane looks up its own.
 template <class T, int HD, bool RUN16>
@@ -447,7 +455,7 @@ __global__ __launch_bounds__(256, (DecodeShape<T, HD, RUN16>::kPerCu)) void k_pa
 // loads in flight, and the groups meet in LDS in their order.
 // grid (query heads, rows); THREADS 512, or 128 where two rounds of theirs take all
 // splits and there are many (1,536 (row, head) pairs of 50 splits and less 11.2 -> 5.2
-// us); S <= kMaxSplits.
+// us); S <= kMaxSplits.  Latency-bound: 4.1 us at 66 splits of 32 heads, 5.4 at 121.
 constexpr int kMaxSplits = 256;
 struct JoinArgs {
   const float *po, *pm, *pl;
@@ -571,19 +579,6 @@ struct PromptShape {
   static constexpr int kPerSimd = B16 || HD < 256 ? 2 : 1;  // waves of a SIMD
 };
 
-// One workgroup a (tile of rows, kv head, split of the tile's positions).  A row is
-// one (token, query head of the kv head's group), tokens in order, so that a tile's
-// heads share every key and value it reads; a wave has 32 rows, the columns of its
-// 32x32 matrix instructions.  Tiles of kKeys positions go through two LDS buffers,
-// copied straight from the pages (16 bytes a lane from any address), the next tile
-// while one is multiplied: one barrier a tile.  S^T = K Q^T leaves a lane half the
-// tile's scores of one row, so the row's maximum and sum take one exchange between
-// lane l and l + 32, and the probabilities are the second product's B operand as
-// they stand (positions in the order that the first product left them).  Its A
-// operand, V^T, comes from the untransposed tile by the transposing LDS load
-// (16 bits) or as single values (fp32).
-// LDS rows are stored with their 16-byte chunks exchanged by an XOR with the row
-// number, which spreads every access over all banks.
 // Tile x of a launch, heavy ones first: tiles by their number within their sequence
 // (later ones see more), the sequences' last ones first.  Tile number l is preceded by
 // count(l + 1) tiles, count(l) = sum over sequences of max(0, tiles - l).
@@ -619,6 +614,29 @@ __device__ __forceinline__ void pick_tile(const int *tile0, int seqs, int x, int
   seq += __builtin_ctzll(__ballot((have >> lane & 1) && __builtin_popcountll(below) == rank));
 }
 
+// One workgroup a (tile of rows, kv head, split of the tile's positions).  A row is
+// one (token, query head of the kv head's group), tokens in order, so that a tile's
+// heads share every key and value it reads; a wave has C of them, the columns of its
+// C x C matrix instructions, C = 32, or 16 for 16-bit heads of 256 (PromptShape; there
+// 8,682 tokens took 950 us at 32 rows and one wave a SIMD, 841 at 16 and two).  Tiles
+// of kKeys positions go through two LDS buffers, copied straight from the pages (16
+// bytes a lane from any address), the next tile while one is multiplied: one barrier a
+// tile.  S^T = K Q^T leaves a lane 1 / NG of the tile's scores of one row, so the
+// row's maximum and sum take one exchange between the NG = 64 / C lanes of a column,
+// and the probabilities are the second product's B operand as they stand (positions in
+// the order that the first product left them).  Its A operand, V^T, comes from the
+// untransposed tile by the transposing LDS load (16 bits) or as single values (fp32).
+// LDS rows are stored with their 16-byte chunks exchanged by an XOR with the row
+// number, which spreads every access over all banks (no conflicts counted; 841 -> 772
+// us with the order of tiles).
+// MFMA-bound, with the softmax between a wave's two products: 8,682 bf16 tokens of 32
+// query heads on 2 kv heads x 256 in three prompts (546 GFLOP) 700 to 785 us as the
+// card's clock goes, 700 to 780 TFLOP/s, where the library's 8192^3 bf16 product
+// reaches 1,186; head dim 128 820 TFLOP/s.  9 short prompts 14.6 us: the longest
+// one's chain of tiles.  14 drafted tokens behind 20,000 positions, split 32 ways, 36 us
+// and 5.7 of join.  fp32, head dim 256: 60 of the 154 TFLOP/s the fp32 library product
+// reaches (one wave a SIMD, outputs in half of the registers).
+// Probabilities are rounded to 16 bits for the second product as in the decode kernel.
 // RUN: pages hold whole runs of the WR positions that a wave copies, whose page is
 // then looked up once, by a scalar load.
 template <class T, int HD, bool RUN>
