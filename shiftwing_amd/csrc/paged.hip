@@ -63,9 +63,20 @@ struct alignas(sizeof(T) * E) Pack {
   T v[E];
 };
 
+// Stores of 16 bytes a lane past the caches (6,379 fp32 tokens 64 -> 51 us, and what
+// reads them next is faster too: 3,000 tokens with their prompt attention 135 -> 130, with
+// a decode 43 -> 35); smaller ones gain nothing (bf16 heads of 256 24.3 and 23.8).
+template <class P>
+__device__ __forceinline__ void store_once(P *to, const P &x) {
+  if constexpr (sizeof(P) == 16)
+    __builtin_nontemporal_store(__builtin_bit_cast(v4u, x), (v4u *)to);
+  else
+    *to = x;
+}
+
 // One workgroup a (token, run of heads), one wave a head: E = HD / 64 elements a
 // lane.  HBM-bound (each value read and written once): 6,379 fp32 tokens of 16 + 2
-// heads of 256 (261 MB) 54 us, 4.8 TB/s, where a large copy reaches 5.1; one bf16
+// heads of 256 (261 MB) 51 us, 5.1 TB/s, a large copy's rate; one bf16
 // token 4.2 us, the launch and its chain of loads.  The angle is formed once a
 // workgroup: turns = position * freq in 64 bits, the whole turns dropped, the rest
 // to fp32 (2^-25 turns), so far positions keep theirs.  The rotation's partners meet
@@ -133,10 +144,10 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 #pragma unroll
     for (int e = 0; e < E; e++) out.v[e] = (T)x[e];
     if (isq) {
-      *(P *)((T *)a.q_out + ((size_t)t * a.nh + h) * HD + E * lane) = out;
+      store_once((P *)((T *)a.q_out + ((size_t)t * a.nh + h) * HD + E * lane), out);
     } else {
-      *(P *)((T *)a.k_pool + at + (size_t)kvh * HD + E * lane) = out;
-      *(P *)((T *)a.v_pool + at + (size_t)kvh * HD + E * lane) = vin;
+      store_once((P *)((T *)a.k_pool + at + (size_t)kvh * HD + E * lane), out);
+      store_once((P *)((T *)a.v_pool + at + (size_t)kvh * HD + E * lane), vin);
     }
   }
 }
@@ -171,9 +182,11 @@ __device__ __forceinline__ v4f mfma_f32_16(float a, float b, v4f c) {
 // Nothing goes through LDS until the waves' merge.  HBM-bound: a block's keys are
 // loaded as soon as the last ones' registers are free, its values likewise, so that a
 // wave always has one of them in flight.  Every key and value is fetched once (466 MB
-// counted for 466 MB): 227,641 bf16 positions of 2 kv heads x 256 83 us, 5.6 TB/s; 48
-// fp16 sequences up to 9,001 at 8 x 128 142 us, 5.1 TB/s; 13 fp32 ones up to 6,000 27
-// us, 5.2 TB/s; one of 4,097 positions 8.5 us, of which 1.6 would be the bytes' own.
+// counted for 466 MB): 227,641 bf16 positions of 2 kv heads x 256 78 us, 6.0 TB/s; 48
+// fp16 sequences up to 9,001 at 8 x 128 136 us, 5.4 TB/s; 13 fp32 ones up to 6,000 30
+// us, 4.6 TB/s; one of 4,097 positions 9.6 us, of which 1.6 would be the bytes' own.
+// The loads leave nothing in the caches: 147 -> 141 and 87 -> 84 us with the join for the
+// first two, 12.0 -> 12.4 for the last, whose keys a repeated call finds there.
 // A probability is rounded to the cache's 16 bits for the second product, half a step
 // of what the values themselves are rounded to; fp32 caches take fp32 products.
 // RUN16: pages hold whole runs of 16 positions, whose page the wave then looks up
@@ -250,7 +263,7 @@ __global__ __launch_bounds__(256, (DecodeShape<T, HD, RUN16>::kPerCu)) void k_pa
       else
         kp = kc + (l.k[b] >= 0 ? l.k[b] : 0);
 #pragma unroll
-      for (int i = 0; i < KR; i++) kr[b][i] = *(const v4u *)(kp + (64 / sizeof(T)) * i + (16 / sizeof(T)) * kg);
+      for (int i = 0; i < KR; i++) kr[b][i] = __builtin_nontemporal_load((const v4u *)(kp + (64 / sizeof(T)) * i + (16 / sizeof(T)) * kg));
     }
   };
   auto load_values = [&](const Loc &l, int key0) {
@@ -266,7 +279,7 @@ __global__ __launch_bounds__(256, (DecodeShape<T, HD, RUN16>::kPerCu)) void k_pa
           vp = vc + (l.v[b][j] >= 0 ? l.v[b][j] : 0);
         vp += W * n;
 #pragma unroll
-        for (int w = 0; w < NW; w++) vr[b][j][w] = *(const VL *)(vp + 16 * W * w);
+        for (int w = 0; w < NW; w++) vr[b][j][w] = __builtin_nontemporal_load((const VL *)(vp + 16 * W * w));
       }
   };
 
@@ -630,8 +643,8 @@ __device__ __forceinline__ void pick_tile(const int *tile0, int seqs, int x, int
 // number, which spreads every access over all banks (no conflicts counted; 841 -> 772
 // us with the order of tiles).
 // MFMA-bound, with the softmax between a wave's two products: 8,682 bf16 tokens of 32
-// query heads on 2 kv heads x 256 in three prompts (546 GFLOP) 700 to 785 us as the
-// card's clock goes, 700 to 780 TFLOP/s, where the library's 8192^3 bf16 product
+// query heads on 2 kv heads x 256 in three prompts (546 GFLOP) 680 to 785 us as the
+// card's clock goes, 700 to 800 TFLOP/s, where the library's 8192^3 bf16 product
 // reaches 1,186; head dim 128 820 TFLOP/s.  9 short prompts 14.6 us: the longest
 // one's chain of tiles.  14 drafted tokens behind 20,000 positions, split 32 ways, 36 us
 // and 5.7 of join.  fp32, head dim 256: 60 of the 154 TFLOP/s the fp32 library product
