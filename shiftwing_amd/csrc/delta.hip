@@ -70,21 +70,21 @@ struct DeltaArgs {
   int chunk0[kSeqs + 1];  // records of sequence s: chunk0[s] .. chunk0[s + 1] - 1
 };
 
+// The next bf16 part of two values, packed, and what is left of them: one conversion
+// for both, whose halves are fp32 values as they stand.
+__device__ __forceinline__ unsigned next_part(float &x, float &y) {
+  const unsigned b = pack2<__bf16>(x, y);
+  x -= __uint_as_float(b << 16);
+  y -= __uint_as_float(b & 0xffff0000u);
+  return b;
+}
 // x as three bf16 values, packed two by two
 __device__ __forceinline__ void split3(const float (&x)[4], v2u (&p)[3]) {
-  float r[4];
-#pragma unroll
-  for (int e = 0; e < 4; e++) r[e] = x[e];
+  float r[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
   for (int k = 0; k < 3; k++) {
-    __bf16 h[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      h[e] = (__bf16)r[e];
-      r[e] -= (float)h[e];
-    }
-    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
-    p[k] = v2u{__builtin_bit_cast(unsigned, v2b{h[0], h[1]}), __builtin_bit_cast(unsigned, v2b{h[2], h[3]})};
+    p[k][0] = next_part(r[0], r[1]);
+    p[k][1] = next_part(r[2], r[3]);
   }
 }
 template <class T>
@@ -611,13 +611,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
       for (int p = 0; p < NP; p++) {
         v4u w;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          typedef __bf16 v2b __attribute__((ext_vector_type(2)));
-          const v2b b = v2b{(__bf16)x[2 * e], (__bf16)x[2 * e + 1]};
-          x[2 * e] -= (float)b[0];
-          x[2 * e + 1] -= (float)b[1];
-          w[e] = __builtin_bit_cast(unsigned, b);
-        }
+        for (int e = 0; e < 4; e++) w[e] = next_part(x[2 * e], x[2 * e + 1]);
         *(v4u *)(to + p * L::kRows) = w;
       }
     }
