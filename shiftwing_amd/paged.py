@@ -13,7 +13,7 @@ import numpy as np
 
 from .abi import ColiPaged
 
-__all__ = ["KINDS", "PagedCache", "from_kind", "to_kind"]
+__all__ = ["KINDS", "PagedCache", "from_kind", "shaped", "to_kind"]
 
 KINDS = {"f32": 0, "f16": 1, "bf16": 2}
 
@@ -36,6 +36,19 @@ def from_kind(a, kind):
     return a.astype(np.float32)
 
 
+def shaped(what, a, shape):
+    """ValueError unless array a has the shape; the C calls take the sizes on trust."""
+    if np.shape(a) != tuple(shape):
+        raise ValueError(f"{what} has shape {np.shape(a)}, not {tuple(shape)}")
+
+
+def packed(start, sequences, rows):
+    """ValueError unless start names rows of that many sequences within the tensors' rows."""
+    if len(start) != sequences + 1 or (sequences and start[-1] > rows):
+        raise ValueError(f"start of {len(start)} entries up to {start[-1] if len(start) else 0} for {sequences} sequences "
+                         f"in {rows} rows")
+
+
 def word(kind):
     """The numpy type of one element."""
     return {"f32": np.float32, "f16": np.float16, "bf16": np.uint16}[kind]
@@ -51,7 +64,7 @@ class PagedCache:
     """Key and value pools of `pages` pages and the page table of `sequences` sequences."""
 
     def __init__(self, be, *, kind, query_heads, kv_heads, head_dim, page_size, pages, table_pages, sequences):
-        self.be, self.kind = be, kind
+        self.be, self.kind, self.sequences = be, kind, sequences
         self.nh, self.nkv, self.hd, self.page_size = query_heads, kv_heads, head_dim, page_size
         self.shape = (pages, page_size, kv_heads, head_dim)
         self.c = ColiPaged(KINDS[kind], query_heads, kv_heads, head_dim, page_size, pages, table_pages,
@@ -62,6 +75,7 @@ class PagedCache:
 
     def set_table(self, table):
         """Page ids [sequences][table_pages]; ids outside the pool name no page."""
+        shaped("table", table, (self.sequences, self.c.table_pages))
         self.table = self.be.upload(np.ascontiguousarray(table, np.int32))
 
     def _put(self, a):
@@ -76,6 +90,15 @@ class PagedCache:
         be = self.be
         start, hs = ints(start)
         length, hl = ints(length)
+        rows = np.shape(k)[0]
+        self._fits(length)
+        packed(start, len(length), rows)
+        for what, x, heads in (("k", k, self.nkv), ("v", v, self.nkv), ("q", q, self.nh)):
+            if x is not None:
+                shaped(what, x, (rows, heads, self.hd))
+        for what, x in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if x is not None:
+                shaped(what, x, (self.hd,))
         dk, dv = self._put(k), self._put(v)
         dq = self._put(q) if q is not None else None
         out = be.upload(np.zeros(np.shape(q), word(self.kind))) if q is not None else None
@@ -99,11 +122,21 @@ class PagedCache:
         Rows of no sequence come back zero."""
         return self._attend("coli_cuda_paged_prompt", q, (start,), length, scale, gate)
 
+    def _fits(self, length):
+        if len(length) > self.sequences:
+            raise ValueError(f"{len(length)} sequences, more than the table's {self.sequences}")
+
     def _attend(self, name, q, start, length, scale, gate):
         be = self.be
         rows = np.shape(q)[0]
         length, hl = ints(length)
         start = [ints(s) for s in start]
+        self._fits(length)
+        if start:
+            packed(start[0][0], len(length), rows)
+        shaped("q", q, (rows if start else len(length), self.nh, self.hd))
+        if gate is not None:
+            shaped("gate", gate, np.shape(q))
         dq, dg = self._put(q), self._put(gate) if gate is not None else None
         out = be.upload(np.zeros((rows, self.nh, self.hd), word(self.kind)))
         be.check(getattr(be.lib, name)(
@@ -117,4 +150,6 @@ class PagedCache:
 
     def write(self, k, v):
         """Both pools whole."""
+        shaped("k", k, self.shape)
+        shaped("v", v, self.shape)
         self.k_pool, self.v_pool = self._put(k), self._put(v)

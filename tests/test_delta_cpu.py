@@ -70,3 +70,22 @@ def test_prompt_rows():
     _refused(_prompt(start=[0, 5, 4]), "sequence 1")
     _refused(_prompt(start=[0, 5, (1 << 31) - 64]), "sequence 1")
     _refused(_prompt(start=[0, 5, (1 << 31) - 65]), "null context")
+
+
+def test_shapes_that_do_not_fit():
+    import numpy as np
+
+    from shiftwing_amd.delta import DeltaRule
+    from test_paged_cpu import _NoDevice
+
+    def rule(heads=4):
+        return DeltaRule(_NoDevice(), kind="f32", key_heads=2, value_heads=4, key_dim=64, value_dim=32, slots=3,
+                         a_log=np.zeros(heads), dt_bias=np.zeros(heads))
+    r, x, a = rule(), np.zeros((5, 2 * 128 + 128)), np.zeros((5, 4))
+    calls = [lambda: rule(3), lambda: r.write(np.zeros((3, 4, 32, 64))), lambda: r.prompt(x, a, a, [0, 6], [0]),
+             lambda: r.prompt(x, a, a, [0, 5], [0, 1]), lambda: r.prompt(x[:, 1:], a, a, [0, 5], [0]),
+             lambda: r.prompt(x, a[:4], a, [0, 5], [0]), lambda: r.prompt(x, a, a[:, :2], [0, 5], [0]),
+             lambda: r.step(x, a, a, [0, 1]), lambda: r.step(x[:2], a, a, [0, 1])]
+    for call in calls:
+        with pytest.raises(ValueError):
+            call()

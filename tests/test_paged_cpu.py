@@ -142,3 +142,34 @@ def test_largest_sizes():
     heads = dict(query_heads=1024, kv_heads=2, **most)  # 512 a kv head: 2^20 tokens of 1,024 heads
     _refused(_prompt(_cache(**heads), start=[0, 1 << 19, (1 << 19) + 1], length=[1 << 20, 1]), "2^29")
     _refused(_prompt(_cache(**heads), start=[0, 1 << 18, 1 << 19], length=[1 << 20, 1 << 20]), "null context")
+
+
+class _NoDevice:
+    """Takes uploads and fails any call: what the wrapper checks, it checks before one."""
+
+    class lib:
+        pass
+
+    ctx = None
+
+    def upload(self, a):
+        return None
+
+
+def test_shapes_that_do_not_fit():
+    import numpy as np
+
+    from shiftwing_amd.paged import PagedCache
+    c = PagedCache(_NoDevice(), kind="bf16", query_heads=4, kv_heads=2, head_dim=64, page_size=16, pages=8, table_pages=4,
+                   sequences=2)
+    k, q = np.zeros((5, 2, 64)), np.zeros((5, 4, 64))
+    calls = [lambda: c.set_table(np.zeros((2, 3), int)), lambda: c.set_table(np.zeros((1, 4), int)),
+             lambda: c.append([0, 3], [3], k, k[:4]), lambda: c.append([0, 6], [6], k, k), lambda: c.append([0], [3], k, k),
+             lambda: c.append([0, 3], [3], k, k, q[:, :3]), lambda: c.append([0, 3], [3], k, k, k_norm=np.ones(63)),
+             lambda: c.append([0, 1, 2, 3], [3, 3, 3], k, k), lambda: c.decode(q[:3], [5, 5, 5], 1.0),
+             lambda: c.decode(q, [5, 5], 1.0), lambda: c.decode(q[:2, :2], [5, 5], 1.0), lambda: c.decode(q[:2], [5, 5], 1.0, q),
+             lambda: c.prompt(q, [0, 6], [6], 1.0), lambda: c.prompt(q, [0, 1, 2], [6], 1.0),
+             lambda: c.prompt(q, [0, 5], [6], 1.0, k), lambda: c.write(k, k)]
+    for call in calls:
+        with pytest.raises(ValueError):
+            call()
