@@ -577,13 +577,17 @@ __device__ __forceinline__ v2u lds_transposed(unsigned at) {
 }
 #pragma clang diagnostic pop
 
-template <class T, int HD>
+template <class T, int HD, int C>
 struct PromptShape {
   static constexpr bool B16 = sizeof(T) == 2;
   // rows of a wave, the columns of its matrix instructions: 32 (32x32x16), or 16
-  // (16x16x32) where the outputs of 32 would leave a SIMD one wave
-  static constexpr int kCols = B16 && HD == 256 ? 16 : 32;
-  static constexpr int kWaves = 128 / kCols;
+  // (16x16x32, 16-bit types), which two waves a SIMD share: where the outputs of 32
+  // would leave it one (head dim 256), and where there are no more workgroups than
+  // compute units, which would leave it one too, with twice the softmax a tile (9 fp16
+  // prompts up to 333 x 12 heads of 64 14.5 -> 12.8 us, 3 bf16 ones up to 200 x 32 of 128
+  // 17.0 -> 13.7; filled, two of 6,000, 118 -> 160 and 440 -> 571)
+  static_assert(C == 32 || (C == 16 && B16), "shapes of the matrix instructions");
+  static constexpr int kWaves = 128 / C;
   static constexpr int kKeys = B16 ? 64 : 32;               // positions of a tile
   static constexpr int kRowBytes = HD * (int)sizeof(T);
   static constexpr int kTileBytes = kKeys * kRowBytes;      // of one matrix
@@ -630,8 +634,8 @@ __device__ __forceinline__ void pick_tile(const int *tile0, int seqs, int x, int
 // One workgroup a (tile of rows, kv head, split of the tile's positions).  A row is
 // one (token, query head of the kv head's group), tokens in order, so that a tile's
 // heads share every key and value it reads; a wave has C of them, the columns of its
-// C x C matrix instructions, C = 32, or 16 for 16-bit heads of 256 (PromptShape; there
-// 8,682 tokens took 950 us at 32 rows and one wave a SIMD, 841 at 16 and two).  Tiles
+// C x C matrix instructions, C = 32 or 16 (PromptShape; at head dim 256 8,682 tokens
+// took 950 us at 32 rows and one wave a SIMD, 841 at 16 and two).  Tiles
 // of kKeys positions go through two LDS buffers, copied straight from the pages (16
 // bytes a lane from any address), the next tile while one is multiplied: one barrier a
 // tile.  S^T = K Q^T leaves a lane 1 / NG of the tile's scores of one row, so the
@@ -645,19 +649,19 @@ __device__ __forceinline__ void pick_tile(const int *tile0, int seqs, int x, int
 // MFMA-bound, with the softmax between a wave's two products: 8,682 bf16 tokens of 32
 // query heads on 2 kv heads x 256 in three prompts (546 GFLOP) 680 to 785 us as the
 // card's clock goes, 700 to 800 TFLOP/s, where the library's 8192^3 bf16 product
-// reaches 1,186; head dim 128 820 TFLOP/s.  9 short prompts 14.6 us: the longest
+// reaches 1,186; head dim 128 820 TFLOP/s.  9 short prompts 12.8 us: the longest
 // one's chain of tiles.  14 drafted tokens behind 20,000 positions, split 32 ways, 36 us
 // and 5.7 of join.  fp32, head dim 256: 60 of the 154 TFLOP/s the fp32 library product
 // reaches (one wave a SIMD, outputs in half of the registers).
 // Probabilities are rounded to 16 bits for the second product as in the decode kernel.
 // RUN: pages hold whole runs of the WR positions that a wave copies, whose page is
 // then looked up once, by a scalar load.
-template <class T, int HD, bool RUN>
-__global__ __launch_bounds__((64 * PromptShape<T, HD>::kWaves), (PromptShape<T, HD>::kPerSimd)) void k_paged_prompt(PromptArgs a) {
-  typedef PromptShape<T, HD> Sh;
+template <class T, int HD, bool RUN, int C>
+__global__ __launch_bounds__((64 * PromptShape<T, HD, C>::kWaves), (PromptShape<T, HD, C>::kPerSimd)) void k_paged_prompt(PromptArgs a) {
+  typedef PromptShape<T, HD, C> Sh;
   constexpr bool B16 = Sh::B16;
   constexpr int KT = Sh::kKeys, RB = Sh::kRowBytes, CPR = RB / 16, NI = Sh::kTileBytes / 1024 / Sh::kWaves;
-  constexpr int C = Sh::kCols, NG = 64 / C, NA = C * C / 64;  // lane groups, registers of a C x C result
+  constexpr int NG = 64 / C, NA = C * C / 64;  // lane groups, registers of a C x C result
   constexpr int NS = KT / C, ND = HD / C;                     // tiles of positions, of dims
   constexpr int KC = CPR / NG;                                // 16-byte chunks of a lane's part of a row
   typedef float Acc __attribute__((ext_vector_type(NA)));     // register i: row 4 NG (i / 4) + 4 g + i % 4
@@ -1137,27 +1141,38 @@ void launch_join(const JoinArgs &a, int hd, int splits, int rows, hipStream_t st
     launch_join<T, 256>(a, splits, grid, st);
 }
 
-template <class T, int HD, bool RUN>
+template <class T, int HD, bool RUN, int C>
 int launch_prompt(const char *name, const PromptArgs &a, dim3 grid, hipStream_t st) {
-  typedef PromptShape<T, HD> Sh;
+  typedef PromptShape<T, HD, C> Sh;
   const hipError_t e =
-      hipFuncSetAttribute((const void *)k_paged_prompt<T, HD, RUN>, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds);
+      hipFuncSetAttribute((const void *)k_paged_prompt<T, HD, RUN, C>, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds);
   if (e != hipSuccess) return fail_hip(name, e);
-  k_paged_prompt<T, HD, RUN><<<grid, 64 * Sh::kWaves, Sh::kLds, st>>>(a);
+  k_paged_prompt<T, HD, RUN, C><<<grid, 64 * Sh::kWaves, Sh::kLds, st>>>(a);
   return 0;
 }
-template <class T, int HD>
+template <class T, int HD, int C>
 int launch_prompt(const char *name, const PromptArgs &a, dim3 grid, hipStream_t st) {
-  typedef PromptShape<T, HD> Sh;
-  return a.map.page_size % (Sh::kKeys / Sh::kWaves) == 0 ? launch_prompt<T, HD, true>(name, a, grid, st)
-                                                         : launch_prompt<T, HD, false>(name, a, grid, st);
+  typedef PromptShape<T, HD, C> Sh;
+  return a.map.page_size % (Sh::kKeys / Sh::kWaves) == 0 ? launch_prompt<T, HD, true, C>(name, a, grid, st)
+                                                         : launch_prompt<T, HD, false, C>(name, a, grid, st);
 }
-constexpr int kPromptRows = PromptShape<float, 64>::kRows;
-static_assert(PromptShape<__bf16, 256>::kRows == kPromptRows, "rows of a tile, the same for all");
+// few: no more workgroups than compute units
+template <class T, int HD>
+int launch_prompt(const char *name, const PromptArgs &a, bool few, dim3 grid, hipStream_t st) {
+  if constexpr (sizeof(T) == 4)
+    return launch_prompt<T, HD, 32>(name, a, grid, st);
+  else if constexpr (HD == 256)
+    return launch_prompt<T, HD, 16>(name, a, grid, st);
+  else
+    return few ? launch_prompt<T, HD, 16>(name, a, grid, st) : launch_prompt<T, HD, 32>(name, a, grid, st);
+}
+constexpr int kPromptRows = PromptShape<float, 64, 32>::kRows;
+static_assert(PromptShape<__bf16, 256, 16>::kRows == kPromptRows, "rows of a tile, the same for all");
 template <class T>
-int launch_prompt(const char *name, const PromptArgs &a, int hd, dim3 grid, hipStream_t st) {
-  return hd == 64 ? launch_prompt<T, 64>(name, a, grid, st)
-                  : hd == 128 ? launch_prompt<T, 128>(name, a, grid, st) : launch_prompt<T, 256>(name, a, grid, st);
+int launch_prompt(const char *name, const PromptArgs &a, int hd, bool few, dim3 grid, hipStream_t st) {
+  return hd == 64    ? launch_prompt<T, 64>(name, a, few, grid, st)
+         : hd == 128 ? launch_prompt<T, 128>(name, a, few, grid, st)
+                     : launch_prompt<T, 256>(name, a, few, grid, st);
 }
 int prompt_keys(int type) { return type != COLI_TYPE_F32 ? 64 : 32; }
 
@@ -1402,9 +1417,10 @@ extern "C" int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *c, void *o
     a.po = a.pm = a.pl = nullptr;
     if (a.splits > 1 && partials(ctx, name, (size_t)a.splits * rows, nh, hd, &a.po, &a.pm, &a.pl)) return -1;
     const dim3 grid((unsigned)(tiles * c->kv_heads), 1, a.splits);
-    const int rc = c->type == COLI_TYPE_F32   ? launch_prompt<float>(name, a, hd, grid, ctx->stream)
-                   : c->type == COLI_TYPE_F16 ? launch_prompt<_Float16>(name, a, hd, grid, ctx->stream)
-                                              : launch_prompt<__bf16>(name, a, hd, grid, ctx->stream);
+    const bool few = tiles * c->kv_heads <= cus_of(ctx);  // the splits fill no more than the compute units
+    const int rc = c->type == COLI_TYPE_F32   ? launch_prompt<float>(name, a, hd, few, grid, ctx->stream)
+                   : c->type == COLI_TYPE_F16 ? launch_prompt<_Float16>(name, a, hd, few, grid, ctx->stream)
+                                              : launch_prompt<__bf16>(name, a, hd, few, grid, ctx->stream);
     if (rc) return -1;
     if (a.splits == 1) continue;
     JoinArgs j;

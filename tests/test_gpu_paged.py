@@ -352,6 +352,29 @@ def test_prompt_more_sequences_than_a_launch(be):
             _check(got[r], want, tol, f"row {r} of sequence {s}")
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,ps", [(64, 16), (64, 5), (128, 16), (128, 5)])
+def test_prompt_more_tiles_than_compute_units(be, kind, hd, ps):
+    """96 kv heads x 4 tiles of rows, which no smaller case has: every ninth row is looked at, and the last."""
+    rng = np.random.default_rng(96)
+    nh, nkv, start, lens = 192, 96, [0, 100, 161], [100, 130]
+    c, table = _cache(be, kind, nh, nkv, hd, ps, lens, rng)
+    K, V = _fill(c, table, lens, rng, kind)
+    V[table[1, 125 // ps], 125 % ps, :, 3] = np.nan  # seen by the last rows alone
+    clean = np.where(np.isnan(V), 0, V)
+    c.write(K, V)
+    q, gate = (_round(rng.standard_normal((161, nh, hd)), kind) for _ in range(2))
+    print(f"[prompt] {kind} heads {nh}/{nkv} x {hd} page {ps} rows {start}", flush=True)
+    got = c.prompt(q, start, lens, 0.11, gate)
+    for s, n in enumerate(lens):
+        for r in [*range(start[s], start[s + 1], 9), start[s + 1] - 1]:
+            sees = n - (start[s + 1] - r) + 1
+            want, tol = _want(q[r], K, clean, table, s, sees, float(np.float32(0.11)), gate[r], kind)
+            dims = [d for d in range(hd) if d != 3 or s == 0 or sees <= 125]
+            assert len(dims) == hd or np.all(np.isnan(got[r, :, 3]))
+            _check(got[r][:, dims], want[:, dims], tol[:, dims], f"row {r} of sequence {s}")
+
+
 # ---- values that are not finite ---------------------------------------------------------------------------
 
 
