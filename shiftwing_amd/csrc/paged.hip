@@ -872,8 +872,10 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD, C>::kWaves), (PromptShape<
       for (int i = 0; i < NA; i++) bm = fmaxf(bm, sc[b][i]);
     bm = over_groups(bm, [](float x, float y) { return fmaxf(x, y); }) * a.scale;
     // any reference serves the softmax: it follows the maximum only when that has
-    // outgrown it by 2^8, so o is hardly ever rescaled
-    if (__any(bm > m_ref + 8.0f)) {
+    // outgrown it by 2^8, so o is hardly ever rescaled.  The difference is exact where
+    // m_ref + 8 is not: at 2^27, where numbers lie 16 apart, that sum may be 16 more, and
+    // 2^16 is no fp16 probability.
+    if (__any(bm - m_ref > 8.0f)) {
       const float m_new = fmaxf(m_ref, bm), alpha = __builtin_amdgcn_exp2f(m_ref - (m_new == -INFINITY ? 0.0f : m_new));
       m_ref = m_new;
       l_run *= alpha;
