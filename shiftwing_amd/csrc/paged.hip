@@ -5,9 +5,9 @@
 // Attention, both forms: o = sum_j p_j v_j / sum_j p_j, p_j = 2^(s_j - m) over the
 // visible positions j, s_j = scale log2(e) q . k_j, with the running maximum m, the
 // sum and o held in fp32 and rescaled when m grows, so the cache is read once.
-// p is rounded to the cache's 16-bit type for the second product (2^-8 / 2^-11
-// relative a term, what the values themselves carry); an fp32 cache keeps fp32
-// products throughout.
+// p is rounded to the cache's 16-bit type for the second product (bf16 2^-8, fp16
+// 2^-11 relative a term, what the values themselves carry, as far as below() holds it
+// among fp16's normal numbers); an fp32 cache keeps fp32 products throughout.
 #include <hip/hip_runtime.h>
 #include <limits.h>
 #include <math.h>
@@ -20,6 +20,20 @@ namespace sw {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// The m of a row's p_j = 2^(s_j - m), from the largest score.  Any m serves, since
+// numerator and sum share it.  fp16 takes it `lift` below that score: its probabilities
+// then reach 2^lift and are normal numbers down to 2^(-14 - lift) of the largest, where
+// many small ones may be all of the output; below 2^-25, as it were with m the largest
+// score, 100,000 of them behind a position whose values are zero came out as nothing.
+// From 2^20 on, where m itself would be rounded by as much, it is the largest score.
+template <class T>
+__device__ __forceinline__ float below(float most, float lift) {
+  if constexpr (__is_same(T, _Float16))
+    return fabsf(most) < 1048576.0f ? most - lift : most;
+  else
+    return most;
+}
 
 // Where a sequence's positions lie.  Offsets are 64-bit: a pool may hold more
 // than 2^31 elements.
@@ -188,7 +202,8 @@ __device__ __forceinline__ v4f mfma_f32_16(float a, float b, v4f c) {
 // The loads leave nothing in the caches: 147 -> 141 and 87 -> 84 us with the join for the
 // first two, 12.0 -> 12.4 for the last, whose keys a repeated call finds there.
 // A probability is rounded to the cache's 16 bits for the second product, half a step
-// of what the values themselves are rounded to; fp32 caches take fp32 products.
+// of what the values themselves are rounded to; fp16's reach 2^15 and are normal numbers
+// down to 2^-29 of the largest; fp32 caches take fp32 products.
 // RUN16: pages hold whole runs of 16 positions, whose page the wave then looks up
 // once, by a scalar load, a block ahead; otherwise every lane looks up its own.
 template <class T, int HD, bool RUN16>
@@ -371,7 +386,7 @@ __global__ __launch_bounds__(256, (DecodeShape<T, HD, RUN16>::kPerCu)) void k_pa
       for (int j = 0; j < 4; j++) bm = fmaxf(bm, sv[b][j]);
     bm = fmaxf(bm, __shfl_xor(bm, 16));
     bm = fmaxf(bm, __shfl_xor(bm, 32));
-    const float m_new = fmaxf(m_run, bm), m_use = m_new == -INFINITY ? 0.0f : m_new;
+    const float m_new = fmaxf(m_run, below<T>(bm, 15.0f)), m_use = m_new == -INFINITY ? 0.0f : m_new;
     const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
     float ps = 0.0f;  // this lane's positions; the lanes of a head meet at the end
 #pragma unroll
@@ -594,6 +609,8 @@ struct PromptShape {
   static constexpr int kLds = 4 * kTileBytes + 16;          // K and V, two buffers, flags
   static constexpr int kRows = 128;                         // (token, head) rows of a workgroup
   static constexpr int kPerSimd = B16 || HD < 256 ? 2 : 1;  // waves of a SIMD
+  // how far the maximum may outgrow the softmax's reference, in powers of two
+  static constexpr float kLag = __is_same(T, _Float16) ? 2.0f : 8.0f;
 };
 
 // Tile x of a launch, heavy ones first: tiles by their number within their sequence
@@ -653,7 +670,9 @@ __device__ __forceinline__ void pick_tile(const int *tile0, int seqs, int x, int
 // one's chain of tiles.  14 drafted tokens behind 20,000 positions, split 32 ways, 36 us
 // and 5.7 of join.  fp32, head dim 256: 60 of the 154 TFLOP/s the fp32 library product
 // reaches (one wave a SIMD, outputs in half of the registers).
-// Probabilities are rounded to 16 bits for the second product as in the decode kernel.
+// Probabilities are rounded to 16 bits for the second product as in the decode kernel;
+// fp16's reach 2^13 where the reference is new, 2^15 at most, and are normal numbers down
+// to 2^-27 of the largest.
 // RUN: pages hold whole runs of the WR positions that a wave copies, whose page is
 // then looked up once, by a scalar load.
 template <class T, int HD, bool RUN, int C>
@@ -871,11 +890,12 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD, C>::kWaves), (PromptShape<
 #pragma unroll
       for (int i = 0; i < NA; i++) bm = fmaxf(bm, sc[b][i]);
     bm = over_groups(bm, [](float x, float y) { return fmaxf(x, y); }) * a.scale;
+    bm = below<T>(bm, 13.0f);
     // any reference serves the softmax: it follows the maximum only when that has
-    // outgrown it by 2^8, so o is hardly ever rescaled.  The difference is exact where
-    // m_ref + 8 is not: at 2^27, where numbers lie 16 apart, that sum may be 16 more, and
-    // 2^16 is no fp16 probability.
-    if (__any(bm - m_ref > 8.0f)) {
+    // outgrown it by 2^kLag, so o is hardly ever rescaled.  The difference is exact where
+    // m_ref + kLag is not: at 2^27, where numbers lie 16 apart, such a sum may be 16 more,
+    // and 2^16 is no fp16 probability.
+    if (__any(bm - m_ref > Sh::kLag)) {
       const float m_new = fmaxf(m_ref, bm), alpha = __builtin_amdgcn_exp2f(m_ref - (m_new == -INFINITY ? 0.0f : m_new));
       m_ref = m_new;
       l_run *= alpha;
