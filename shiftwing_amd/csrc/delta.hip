@@ -22,12 +22,12 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include "sw_delta_plan.h"
 #include "sw_serve.h"
 
 namespace sw {
 namespace {
 
-constexpr int kChunk = 64;
 constexpr int kKey = 128;   // largest key_dim
 constexpr int kSlice = 32;  // value columns of a k_delta_scan workgroup
 
@@ -530,7 +530,6 @@ __global__ __launch_bounds__(512) void k_delta_scan(DeltaArgs g) {
   const int hk = h / (g.vh / g.kh);
   const int rows = g.rows[s];
   const int c0 = g.chunk_first, c1 = min(c0 + g.chunks, (rows + kChunk - 1) / kChunk);
-  if (c0 > 0 && c0 >= c1) return;  // an earlier pass ended this sequence
   const size_t at = ((size_t)g.slot[s] * g.vh + h) * g.dk * g.dv + col;
   const float *from = c0 > 0 ? g.state_out : g.state;
   v4f S[2];  // rows 32 rt + 16 i + 4 kg + e
@@ -851,12 +850,10 @@ extern "C" int coli_cuda_delta_prompt(ColiCuda *ctx, const ColiDelta *d, void *o
   g.state_out = state_out;
   g.q_stride = d->q_stride, g.k_stride = d->k_stride, g.v_stride = d->v_stride;
   g.kh = d->key_heads, g.vh = d->value_heads, g.dk = d->key_dim, g.dv = d->value_dim;
-  // records of a pass: 512 MiB, a chunk of every sequence at least
   const size_t chunk_bytes = (size_t)g.vh * (d->type == COLI_TYPE_F32 ? Rec<float>::kBytes : Rec<__bf16>::kBytes);
-  for (int s0 = 0; s0 < sequences; s0 += kSeqs) {
-    const int n = sequences - s0 < kSeqs ? sequences - s0 : kSeqs;
-    long long per = (long long)((512u << 20) / chunk_bytes) / n;
-    if (per < 1) per = 1;
+  const int most = delta_sequences(kSeqs, chunk_bytes);
+  for (int s0 = 0; s0 < sequences; s0 += most) {
+    const int n = sequences - s0 < most ? sequences - s0 : most;
     // long sequences first: their walk takes longest
     for (int s = 0; s < n; s++) {
       const int rows = start[s0 + s + 1] - start[s0 + s];
@@ -870,24 +867,24 @@ extern "C" int coli_cuda_delta_prompt(ColiCuda *ctx, const ColiDelta *d, void *o
       g.rows[i] = rows;
       g.slot[i] = slot[s0 + s];
     }
-    const int longest = (int)(((long long)g.rows[0] + kChunk - 1) / kChunk);
-    g.chunks = per < longest ? (int)per : longest;
-    g.seqs = n;
-    for (g.chunk_first = 0; g.chunk_first == 0 || g.chunk_first < longest; g.chunk_first += g.chunks) {
-      for (int s = 0; s < n; s++) {
-        int c = (int)(((long long)g.rows[s] + kChunk - 1) / kChunk) - g.chunk_first;
-        if (c > g.chunks) c = g.chunks;
-        g.chunk0[s + 1] = g.chunk0[s] + (c > 0 ? c : 0);
+    const int longest = (int)chunks_of(g.rows[0]);
+    g.chunk_first = 0;
+    do {  // the first pass takes empty sequences along, which keep their state
+      g.seqs = g.chunk_first ? delta_live(g.rows, n, g.chunk_first) : n;
+      g.chunks = (int)delta_pass(g.rows, n, g.chunk_first, chunk_bytes);
+      for (int s = 0; s < g.seqs; s++) {
+        const int left = (int)chunks_of(g.rows[s]) - g.chunk_first;
+        g.chunk0[s + 1] = g.chunk0[s] + (left < g.chunks ? left : g.chunks);
       }
-      const int chunks = g.chunk0[n];
+      const int chunks = g.chunk0[g.seqs];
       if (ensure_scratch(ctx, kScrDelta, (size_t)(chunks ? chunks : 1) * chunk_bytes, name)) return -1;
       g.rec = (char *)ctx->scratch[kScrDelta];
       const int rc = d->type == COLI_TYPE_F32   ? launch_delta<float>(name, g, chunks, ctx->stream)
                      : d->type == COLI_TYPE_F16 ? launch_delta<_Float16>(name, g, chunks, ctx->stream)
                                                 : launch_delta<__bf16>(name, g, chunks, ctx->stream);
       if (rc) return -1;
-      if (longest == 0) break;
-    }
+      g.chunk_first += g.chunks;
+    } while (g.chunk_first < longest);
   }
   return launch_status(name);
 }
