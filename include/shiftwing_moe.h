@@ -559,7 +559,15 @@ int coli_cuda_moe_stack_drill(ColiCuda *ctx, int absent_workgroups,
 /* No counterpart in the reference backend, whose caches are one fp32 slab a
  * slot and whose Gated DeltaNet advances a handful of tokens a call.  The same
  * conventions: 0 / -1 with a message, device pointers owned by the caller,
- * everything ordered on the context's stream, nothing waited for.
+ * everything ordered on the context's stream.  Nothing is waited for but the
+ * stream itself where a call needs a larger workspace than any before it: the
+ * workspaces grow with room to spare (attention takes up to 64 MiB with its first
+ * split, prompts of the gated delta rule half as much again as they need, up to
+ * 512 MiB), so a serving loop soon stops doing so.
+ * The context's stream does not wait for work on any other stream, nor another
+ * for it: what else writes a call's tensors has to be finished before the call,
+ * and coli_cuda_sync comes before anything else reads its results or frees its
+ * tensors.
  *
  * Element types of the tensors of this part (sums, softmax statistics and
  * recurrent states are fp32 whatever the type). */

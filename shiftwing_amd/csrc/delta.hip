@@ -877,7 +877,8 @@ extern "C" int coli_cuda_delta_prompt(ColiCuda *ctx, const ColiDelta *d, void *o
         g.chunk0[s + 1] = g.chunk0[s] + (left < g.chunks ? left : g.chunks);
       }
       const int chunks = g.chunk0[g.seqs];
-      if (ensure_scratch(ctx, kScrDelta, (size_t)(chunks ? chunks : 1) * chunk_bytes, name)) return -1;
+      const size_t bytes = (size_t)(chunks ? chunks : 1) * chunk_bytes;
+      if (ensure_room(ctx, kScrDelta, bytes, bytes / 2 * 3 < kDeltaRecords ? bytes / 2 * 3 : kDeltaRecords, name)) return -1;
       g.rec = (char *)ctx->scratch[kScrDelta];
       const int rc = d->type == COLI_TYPE_F32   ? launch_delta<float>(name, g, chunks, ctx->stream)
                      : d->type == COLI_TYPE_F16 ? launch_delta<_Float16>(name, g, chunks, ctx->stream)

@@ -1198,10 +1198,18 @@ int launch_prompt(const char *name, const PromptArgs &a, int hd, bool few, dim3 
 }
 int prompt_keys(int type) { return type != COLI_TYPE_F32 ? 64 : 32; }
 
-// Partial records of n (split, row) pairs: outputs, maxima, sums.
+// Partial records of n (split, row) pairs: outputs, maxima, sums.  A decoding loop needs a
+// split more every some hundred tokens, so the first call takes what its heads can come
+// to: (split, row, head) records of 128 rows a compute unit for prompts, of 16 heads a
+// workgroup and three rounds of four workgroups a compute unit for single tokens, and one
+// for each sequence of a launch; 64 MiB at most (14, 28, 55 MB at 32 heads of 64, 128, 256).
 int partials(ColiCuda *ctx, const char *name, size_t n, int nh, int hd, float **po, float **pm, float **pl) {
-  const size_t heads = n * nh;
-  if (ensure_scratch(ctx, kScrPaged, heads * (hd + 2) * sizeof(float), name)) return -1;
+  const size_t heads = n * nh, record = (hd + 2) * sizeof(float), cus = cus_of(ctx);
+  size_t room = 12 * 16 * cus + (size_t)kSeqs * nh;
+  if (room < 128 * cus) room = 128 * cus;
+  room = room * record < (64u << 20) ? room * record : 64u << 20;
+  if (room < heads * record) room = heads * record / 2 * 3;
+  if (ensure_room(ctx, kScrPaged, heads * record, room, name)) return -1;
   *po = (float *)ctx->scratch[kScrPaged];
   *pm = *po + heads * hd;
   *pl = *pm + heads;

@@ -112,6 +112,17 @@ struct OnDevice {
   OnDevice &operator=(const OnDevice &) = delete;
 };
 
+// ensure_scratch for sizes that creep up from call to call: where the slot has to grow,
+// which waits for the stream, it grows to `room`, or to what is needed if that cannot be had.
+inline int ensure_room(ColiCuda *ctx, Scratch which, size_t bytes, size_t room, const char *where) {
+  if (ctx->scratch_cap[which] >= bytes) return 0;
+  if (room > bytes) {
+    if (!ensure_scratch(ctx, which, room, where)) return 0;
+    (void)hipGetLastError();
+  }
+  return ensure_scratch(ctx, which, bytes, where);
+}
+
 inline int type_bytes(int type) { return type == COLI_TYPE_F32 ? 4 : type == COLI_TYPE_F16 || type == COLI_TYPE_BF16 ? 2 : 0; }
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
