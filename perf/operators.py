@@ -11,6 +11,10 @@ dim 64; DeltaNet heads of 128 x 128) and generic ones of head dims 64 and 128.
   gen128 32 query heads over 8 kv heads of 128
   gen64  12 query heads over 12 kv heads of 64
 
+The framework's calls go to the stream of their own context, which no torch stream waits for, nor it for them.  So
+prepare() returns inputs that are finished, and whoever reads the results of run(), or lets go of a state that it has
+run, waits for the device first (torch.cuda.synchronize()).
+
 Lengths of a batch come from the case's `longest` and `sequences` alone (a spread from long to short), so work()
 knows them.
 """
@@ -127,6 +131,13 @@ class _Rand:
 
 
 def prepare(case, seed):
+    torch.cuda.synchronize()  # calls on earlier states, whose memory this one may get
+    s = _inputs(case, seed)
+    torch.cuda.synchronize()  # the inputs, before another stream reads them
+    return s
+
+
+def _inputs(case, seed):
     r, m, dt = _Rand(seed), SHAPES[case["model"]], TYPES[case["type"]]
     new, length = _lengths(case)
     start = [sum(new[:i]) for i in range(len(new) + 1)]
