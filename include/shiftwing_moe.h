@@ -623,8 +623,8 @@ int coli_cuda_paged_append(ColiCuda *ctx, const ColiPaged *cache,
  * the cache, query head h on kv head h / (query_heads / kv_heads), times
  * sigmoid(gate) where gates are given (gate_stride elements from row to row,
  * gate_head_stride from head to head, both multiples of 4, the gates aligned to
- * four elements).  q and out are contiguous and 16-byte aligned, scale is finite
- * (negative or zero too).  Sequences that see nothing get zeros.  What lies in
+ * four elements).  q and out are contiguous and 16-byte aligned, scale * log2(e)
+ * is finite (negative or zero too).  Sequences that see nothing get zeros.  What lies in
  * positions that a row does not see changes nothing, whatever it is; infinities
  * and NaN in those it sees take their course. */
 int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *cache, void *out,

@@ -1288,7 +1288,7 @@ extern "C" int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *c, void *o
       !gate_ok(name, c, gate, gate_stride, gate_head_stride))
     return -1;
   if (!out || !q || !aligned16(out) || !aligned16(q)) return fail_arg("%s: q and out must be 16-byte aligned", name);
-  if (!isfinite(scale)) return fail_arg("%s: scale is not finite", name);
+  if (!isfinite(scale * kLog2e)) return fail_arg("%s: scale, or scale * log2(e), is not finite", name);
   if (!ctx) return fail_arg("%s: null context", name);
   OnDevice on(ctx);
   const int nh = c->query_heads, hd = c->head_dim, size = type_bytes(c->type);
@@ -1399,7 +1399,7 @@ extern "C" int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *c, void *o
   if (sequences && !start) return fail_arg("%s: null start", name);
   if (!rows_ok(name, c, start, length, sequences) || !gate_ok(name, c, gate, gate_stride, gate_head_stride)) return -1;
   if (!out || !q || !aligned16(out) || !aligned16(q)) return fail_arg("%s: q and out must be 16-byte aligned", name);
-  if (!isfinite(scale)) return fail_arg("%s: scale is not finite", name);
+  if (!isfinite(scale * kLog2e)) return fail_arg("%s: scale, or scale * log2(e), is not finite", name);
   const int nh = c->query_heads, hd = c->head_dim, G = nh / c->kv_heads, R = kPromptRows;
   // (token, head) rows of a call, which also bounds a launch's threads: 256 a tile of 128
   // rows, or 512 at head_dim 256
