@@ -55,8 +55,12 @@ def word(kind):
 
 
 def ints(a):
-    """A host array of C ints."""
-    a = np.ascontiguousarray(a, np.int32)
+    """A host array of C ints; ValueError where the values are none, or not in a row."""
+    given = np.asarray(a)
+    with np.errstate(invalid="ignore"):
+        a = np.ascontiguousarray(given.astype(np.int32))
+    if given.ndim != 1 or not np.array_equal(given, a):
+        raise ValueError(f"not a row of C ints: {given}")
     return a, C.c_void_p(a.ctypes.data)
 
 
