@@ -626,7 +626,14 @@ int coli_cuda_paged_append(ColiCuda *ctx, const ColiPaged *cache,
  * four elements).  q and out are contiguous and 16-byte aligned, scale * log2(e)
  * is finite (negative or zero too).  Sequences that see nothing get zeros.  What lies in
  * positions that a row does not see changes nothing, whatever it is; infinities
- * and NaN in those it sees take their course. */
+ * and NaN in those it sees take their course.
+ *
+ * Scores, the softmax's maxima and sums and the outputs until their rounding are
+ * fp32.  The weights are rounded to the cache's type before they multiply the
+ * values: bf16 2^-8, fp16 2^-11 relative, and fp16 ones below 2^-27 of a row's
+ * largest by up to 2^-38 of it; those of fp32 caches are not.  The sums of weighted
+ * values are divided by the sum of weights at the end, so up to 2^8 times the sum of
+ * a row's |values| has to be within fp32. */
 int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *cache, void *out,
                            const void *q, const void *gate,
                            long long gate_stride, int gate_head_stride,
@@ -634,8 +641,10 @@ int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *cache, void *out,
                            const int *table, const int *length, int sequences,
                            float scale);
 /* The same for packed prompts (or chunks of them, or drafted tokens): row i of
- * the n rows of a sequence sees its positions up to length - n + i.  rows *
- * query_heads, in tiles of 128 for each sequence and kv head, at most 2^29. */
+ * the n rows of a sequence sees its positions up to length - n + i.  Infinite or NaN
+ * values that only some rows of a tile see are kept from the others by forming
+ * those anew, which takes long: 1 to 2 ms for each (row, query head) of 16 or 32
+ * that see 5,000 positions.  rows * query_heads, in tiles of 128 for each sequence and kv head, at most 2^29. */
 int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *cache, void *out,
                            const void *q, const void *gate,
                            long long gate_stride, int gate_head_stride,
@@ -661,7 +670,11 @@ int coli_cuda_paged_prompt(ColiCuda *ctx, const ColiPaged *cache, void *out,
  * key_dim a multiple of 8 up to 128, value_dim of 32 up to 256; tensors 16-byte
  * aligned, strides non-negative multiples of 8.
  *
- * Inputs and states are finite, and so are the fp32 sums of squares of q and k.
+ * Products are fp32, formed from the bf16 parts that make up their factors, all
+ * three for fp32 outputs and for states, two (16 bits) for outputs of 16-bit types.
+ *
+ * Inputs, states and e^a_log are finite, and so are the fp32 sums of squares of q and
+ * k; values and states are below 2^127, where bf16 parts end.
  * Otherwise the token's outputs and those after it are NaN where the rule reaches
  * them, and in coli_cuda_delta_prompt, which takes 64 tokens at once, outputs of
  * the same value head up to 63 tokens before it may be NaN too; other sequences

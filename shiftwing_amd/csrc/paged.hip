@@ -90,7 +90,8 @@ __device__ __forceinline__ void store_once(P *to, const P &x) {
 
 // One workgroup a (token, run of heads), one wave a head: E = HD / 64 elements a
 // lane.  HBM-bound (each value read and written once): 6,379 fp32 tokens of 16 + 2
-// heads of 256 (261 MB) 51 us, 5.1 TB/s, a large copy's rate; one bf16
+// heads of 256 (261 MB) 51 us, 5.1 TB/s, a large copy's rate (41 in calls on the same
+// tokens, which the memory-side cache then holds); one bf16
 // token 4.2 us, the launch and its chain of loads.  The angle is formed once a
 // workgroup: turns = position * freq in 64 bits, the whole turns dropped, the rest
 // to fp32 (2^-25 turns), so far positions keep theirs.  The rotation's partners meet
@@ -195,10 +196,11 @@ __device__ __forceinline__ v4f mfma_f32_16(float a, float b, v4f c) {
 // row n of dim tile d stands for dim W n + d (tiles of one load).
 // Nothing goes through LDS until the waves' merge.  HBM-bound: a block's keys are
 // loaded as soon as the last ones' registers are free, its values likewise, so that a
-// wave always has one of them in flight.  Every key and value is fetched once (466 MB
-// counted for 466 MB): 227,641 bf16 positions of 2 kv heads x 256 78 us, 6.0 TB/s; 48
-// fp16 sequences up to 9,001 at 8 x 128 136 us, 5.4 TB/s; 13 fp32 ones up to 6,000 30
-// us, 4.6 TB/s; one of 4,097 positions 9.6 us, of which 1.6 would be the bytes' own.
+// wave always has one of them in flight.  Every key and value is fetched once (471 MB
+// counted for 466 MB) by each group of 16 query heads of its kv head.  Kernel times:
+// 227,641 bf16 positions of 2 kv heads x 256 79 us, 5.9 TB/s; 48
+// fp16 sequences up to 9,001 at 8 x 128 137 us, 5.3 TB/s; 13 fp32 ones up to 6,000 31
+// us, 4.5 TB/s; one of 4,097 positions 10 us, of which 1.6 would be the bytes' own.
 // The loads leave nothing in the caches: 147 -> 141 and 87 -> 84 us with the join for the
 // first two, 12.0 -> 12.4 for the last, whose keys a repeated call finds there.
 // A probability is rounded to the cache's 16 bits for the second product, half a step
@@ -598,9 +600,11 @@ struct PromptShape {
   // rows of a wave, the columns of its matrix instructions: 32 (32x32x16), or 16
   // (16x16x32, 16-bit types), which two waves a SIMD share: where the outputs of 32
   // would leave it one (head dim 256), and where there are no more workgroups than
-  // compute units, which would leave it one too, with twice the softmax a tile (9 fp16
-  // prompts up to 333 x 12 heads of 64 14.5 -> 12.8 us, 3 bf16 ones up to 200 x 32 of 128
-  // 17.0 -> 13.7; filled, two of 6,000, 118 -> 160 and 440 -> 571)
+  // compute units, which would leave it one too, with twice the softmax a tile.  bf16
+  // prompts of one length, 32 against 16 rows, us a call: head dim 64, 120 workgroups 12.5
+  // and 10.6, 240 17.0 and 15.4, then 336 17.8 and 20.4, 432 18.9 and 22.3, 720 44.5 and
+  // 58.1; head dim 128, 192 18.3 and 15.1, then 320 20.9 and 22.6, 640 43.7 and 42.3, 896
+  // 49.2 and 56.4, 1,880 150 and 189; fp16 the same within 2 us
   static_assert(C == 32 || (C == 16 && B16), "shapes of the matrix instructions");
   static constexpr int kWaves = 128 / C;
   static constexpr int kKeys = B16 ? 64 : 32;               // positions of a tile
@@ -663,13 +667,22 @@ __device__ __forceinline__ void pick_tile(const int *tile0, int seqs, int x, int
 // LDS rows are stored with their 16-byte chunks exchanged by an XOR with the row
 // number, which spreads every access over all banks (no conflicts counted; 841 -> 772
 // us with the order of tiles).
-// MFMA-bound, with the softmax between a wave's two products: 8,682 bf16 tokens of 32
-// query heads on 2 kv heads x 256 in three prompts (546 GFLOP) 680 to 785 us as the
-// card's clock goes, 700 to 800 TFLOP/s, where the library's 8192^3 bf16 product
-// reaches 1,186; head dim 128 820 TFLOP/s.  9 short prompts 12.8 us: the longest
-// one's chain of tiles.  14 drafted tokens behind 20,000 positions, split 32 ways, 36 us
-// and 5.7 of join.  fp32, head dim 256: 60 of the 154 TFLOP/s the fp32 library product
-// reaches (one wave a SIMD, outputs in half of the registers).
+// 8,682 bf16 tokens of 32 query heads on 2 kv heads x 256 in three prompts (546 GFLOP)
+// 690 us a call, 790 TFLOP/s (755 under the profiler), where the library's 8192^3 bf16
+// product reaches 1,186.  No unit is full: counted, the matrix units are busy for 35% of
+// the cycles and LDS for as many, since with 16 rows a matrix instruction of 16 cycles
+// takes a fragment of 1 KB of its own; two waves a SIMD do not overlap the rest, a tile's
+// products, softmax and barrier in turn.  32 rows at head dim 128 (43% and 22%) 376 us
+// for two prompts of 6,000 and 2,121, 880 TFLOP/s.  9 short prompts 12.6 us: the longest
+// one's chain of tiles.  14 drafted tokens behind 20,000 positions, split 32 ways, 36 to
+// 41 us, 4 TB/s: ten tiles a workgroup in turn, in which 18 of 32 waves multiply rows
+// that do not exist; 5.8 of join.  fp32, two prompts of 1,999 and 706 tokens, 16 heads of
+// 256: 59 of the 154 TFLOP/s the fp32 library product reaches; matrix units busy for 69%
+// of the cycles of a busy compute unit, which holds one wave a SIMD and one of 340
+// workgroups of unequal length.
+// Registers: the 32-row 16-bit kernels at head dim 128 spill 2 or 3 of theirs; of the
+// fp32 ones, head dim 256 spills 4 (34 where pages do not hold whole runs), head dim 128
+// 189 on such pages.
 // Probabilities are rounded to 16 bits for the second product as in the decode kernel;
 // fp16's reach 2^13 where the reference is new, 2^15 at most, and are normal numbers down
 // to 2^-27 of the largest.
@@ -966,7 +979,10 @@ __global__ __launch_bounds__((64 * PromptShape<T, HD, C>::kWaves), (PromptShape<
   // A position of a tile that a row does not see has the probability zero, and zero times
   // an infinite or NaN value is NaN.  Rows of the wave that are not finite are formed anew
   // from what they see, one by one, if one of the positions unseen by the first row
-  // holds such a value: nothing any ordinary prompt pays for.
+  // holds such a value: nothing any ordinary prompt pays for.  Where it runs, one wave
+  // takes 1 to 2 ms a row and 5,000 positions: a NaN value in the last position of
+  // prompts of 5,000 to 6,000 tokens 0.69 -> 35 ms (16 rows) and 0.43 -> 42 (32); in the
+  // first, which every row sees, no more than without.
   float zero = 0.0f;
 #pragma unroll
   for (int d = 0; d < ND; d++)
@@ -1317,8 +1333,8 @@ extern "C" int coli_cuda_paged_decode(ColiCuda *ctx, const ColiPaged *c, void *o
     }
     // All splits of one length, in blocks of the four waves.  Where a compute unit holds
     // one workgroup, the least length whose workgroups all run at once: 13 fp32
-    // sequences up to 6,000 positions 26 us, in two and three rounds 36 and 44; three
-    // bf16 ones up to 131,071 82 against 86 and 89.  Where it holds several (or one
+    // sequences up to 6,000 positions 31 us and 4.6 of join, in two and three rounds 41 and
+    // 48; three bf16 ones up to 131,071 79 and 4.8, against 83 and 6.4, 91 and 7.6.  Where it holds several (or one
     // round leaves the longest split half as much again as an even share, beside many
     // short sequences), a third of an even share, in rounds that level out: 48 fp16
     // sequences up to 9,001 at head dim 128 160 us in one round, 145 / 143 / 143 at a
