@@ -562,8 +562,8 @@ int coli_cuda_moe_stack_drill(ColiCuda *ctx, int absent_workgroups,
  * everything ordered on the context's stream.  Nothing is waited for but the
  * stream itself where a call needs a larger workspace than any before it: the
  * workspaces grow with room to spare (attention takes up to 64 MiB with its first
- * split, prompts of the gated delta rule half as much again as they need, up to
- * 512 MiB), so a serving loop soon stops doing so.
+ * split; beyond that, and for prompts of the gated delta rule up to 512 MiB, half as
+ * much again as the call needs), so a serving loop soon stops doing so.
  * The context's stream does not wait for work on any other stream, nor another
  * for it: what else writes a call's tensors has to be finished before the call,
  * and coli_cuda_sync comes before anything else reads its results or frees its
